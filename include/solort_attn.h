@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define SOLORT_ATTN_ABI_VERSION 3
+#define SOLORT_ATTN_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define SOLORT_API __attribute__((visibility("default")))
@@ -400,11 +400,132 @@ typedef struct SolortGemvArgs {
 
 SOLORT_API int solort_attn_gemv(const SolortGemvArgs* args, void* stream);
 
+/*
+ * The paged KV cache held in 4 bits: the same pages, slots and block tables as the bf16 arena, 160
+ * bytes per token and KV head instead of 512. A row of 128 values is held in four groups of 32 as
+ *   mid + scale * (code - 7.5), code in 0..15,
+ *   mid = bf16((lo + hi) / 2), scale = bf16, rounded up, of max(hi - mid, mid - lo) / 7.5,
+ *   code = rint((x - mid) / scale + 7.5)
+ * (lo, hi: the group's least and greatest value; each step fp32), so that every held value is within
+ * scale / 2 of x. A group with an infinity or a NaN is held as NaN.
+ *
+ * One layer's arena: the page p of KV head h is the P * 160 bytes at kv_pages + p*kv_stride_page +
+ * h*kv_stride_head (bytes, multiples of 16), P a power of two >= 8, in blocks of 8 tokens, 1280
+ * bytes each:
+ *   bytes    0..511   key codes: token i at 64 i; 16-byte chunk t, 32-bit word g: nibble j is the
+ *                     code of dim 32 g + 8 t + j
+ *   bytes  512..639   token i at 16 i: word g = bf16 scale (low half) and mid (high half) of group g
+ *   bytes  640..1151  value codes: tokens 2p, 2p + 1 at 128 p; 16-byte unit u (0..7) at place u ^ 2p;
+ *                     word g: low half token 2p, high half token 2p + 1; nibble j of a half is the
+ *                     code of dim 32 g + 4 u + j
+ *   bytes 1152..1279  the values' scale and mid, as the keys'
+ * No byte is shared by two tokens. An arena of zero bytes holds zeros.
+ *
+ * Slots are int64, page * P + row, on the device. -1 marks a padded row: nothing is read or written
+ * for it. Any other slot outside the arena is skipped likewise and sets bit 4 of the device status.
+ * Which row stays is not defined where two rows of one call have the same slot.
+ *
+ * solort_attn_qk_norm_rope_append_int4: the attention prologue of a batch. Token i sits at
+ * positions[i] of its sequence (any mix of sequences); from its row of the fused QKV projection,
+ * q_out[i] = bf16(rope(norm(q))), and rope(norm(k)) and v go to slots[i]. Norm and rotation are
+ * SolortPrologueArgs' in fp32 with one rounding at the end. A token whose position has no row in
+ * the tables is skipped and sets bit 4. Pointers 16-byte aligned, strides multiples of 8 elements.
+ * Counterpart of solort_attn_qk_norm_rope_append for src/solort/model/cuda_graph_executor.py:176-179.
+ */
+typedef struct SolortInt4AppendArgs {
+  const void* qkv;
+  int64_t qkv_stride_token;
+  int32_t num_tokens, num_qo_heads, num_kv_heads, head_dim;
+  const void* q_norm_weight;
+  const void* k_norm_weight;
+  float eps;
+  const void* cos; /* bf16 [rope_rows, 128], as sin */
+  const void* sin;
+  int64_t rope_stride;
+  int32_t rope_rows;
+  const int64_t* positions;
+  const int64_t* slots;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head;
+  void* kv_pages;
+  int64_t kv_stride_page, kv_stride_head; /* bytes */
+  int32_t page_size, num_pages;
+} SolortInt4AppendArgs;
+
+SOLORT_API int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* args, void* stream);
+
+/* Store: token i's K and V rows (bf16, head h at + h*stride_head) to slots[i]. The 4-bit form of
+ * solort_attn_kv_store (src/solort/cache/kv_cache.py:191-235). */
+typedef struct SolortInt4StoreArgs {
+  const void* key;
+  const void* value;
+  int64_t key_stride_token, key_stride_head, value_stride_token, value_stride_head;
+  int32_t num_tokens, num_kv_heads, head_dim;
+  const int64_t* slots;
+  void* kv_pages;
+  int64_t kv_stride_page, kv_stride_head; /* bytes */
+  int32_t page_size, num_pages;
+} SolortInt4StoreArgs;
+
+SOLORT_API int solort_attn_kv_store_int4(const SolortInt4StoreArgs* args, void* stream);
+
+/* Load: the held values at slots[i], rounded to bf16, to row i of key and value: the gather of
+ * src/solort/cache/kv_cache.py:237-256. Feeds solort_attn_prefill a cached prefix. */
+typedef struct SolortInt4LoadArgs {
+  void* key;
+  void* value;
+  int64_t key_stride_token, key_stride_head, value_stride_token, value_stride_head;
+  int32_t num_tokens, num_kv_heads, head_dim;
+  const int64_t* slots;
+  const void* kv_pages;
+  int64_t kv_stride_page, kv_stride_head; /* bytes */
+  int32_t page_size, num_pages;
+} SolortInt4LoadArgs;
+
+SOLORT_API int solort_attn_kv_load_int4(const SolortInt4LoadArgs* args, void* stream);
+
+/*
+ * GQA attention of q_len query tokens per sequence over the 4-bit pages: solort_attn_decode with a
+ * block table (q, out, q_pos, q_lens, max_kv_len, block_table and the SOLORT_DECODE_STABLE_PREFIX
+ * flag as there), for any q_len: the rows of a KV head are taken in blocks of 16. Rows that see no
+ * key are zero; rows past q_lens are not written. Keys behind a block-table entry outside the arena
+ * count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
+ * elements; out 8-byte aligned, multiples of 4. The workspace (256-byte aligned; query its size with
+ * the same args) depends on the device and the row count, not on the lengths or the batch past one
+ * wave of CTAs; calls that share one must be ordered on their streams. num_ctas: 0 = one resident
+ * wave, otherwise the number of CTAs over which the keys are divided.
+ */
+typedef struct SolortInt4DecodeArgs {
+  const void* q;
+  int64_t q_stride_batch, q_stride_token, q_stride_head;
+  void* out;
+  int64_t out_stride_batch, out_stride_token, out_stride_head;
+  const void* kv_pages;
+  int64_t kv_stride_page, kv_stride_head; /* bytes */
+  int32_t page_size, num_pages;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int64_t* q_pos;
+  const int32_t* q_lens;
+  int32_t batch, q_len, num_qo_heads, num_kv_heads, head_dim;
+  int32_t max_kv_len;
+  float scale;
+  int32_t num_ctas;
+  void* workspace;
+  size_t workspace_bytes;
+  uint32_t flags; /* SOLORT_DECODE_* bits */
+} SolortInt4DecodeArgs;
+
+SOLORT_API int solort_attn_decode_int4_workspace_size(const SolortInt4DecodeArgs* args, size_t* bytes);
+SOLORT_API int solort_attn_decode_int4(const SolortInt4DecodeArgs* args, void* stream);
+
 /* Reads and clears the device status word of the current device (bit 0: an in-kernel wait hit
  * its time limit and the kernel returned without writing its output; bit 1: a tensor-memory
  * allocation wait hit its limit; bit 2: a kernel found its shared memory misaligned and returned
  * without writing; bit 3: an exchange merge waited a second for a peer's partial and left the
- * row unwritten; bit 4: solort_attn_kv_store met a slot outside the arena and skipped it). */
+ * row unwritten; bit 4: a slot-mapped call met a slot outside the arena, or a position without a
+ * RoPE row, and skipped it; bit 5: solort_attn_decode_int4 met a block-table entry outside the
+ * arena). */
 SOLORT_API int solort_attn_device_status(unsigned* flags);
 
 SOLORT_API const char* solort_attn_status_string(int code);

@@ -48,6 +48,11 @@ EXPORTED_SYMBOLS = (
     "solort_attn_silu_mul",
     "solort_attn_gemv",
     "solort_attn_kv_store",
+    "solort_attn_qk_norm_rope_append_int4",
+    "solort_attn_kv_store_int4",
+    "solort_attn_kv_load_int4",
+    "solort_attn_decode_int4_workspace_size",
+    "solort_attn_decode_int4",
 )
 
 MAX_RANKS = 8  # SOLORT_MAX_RANKS
@@ -210,6 +215,64 @@ class SolortKVStoreArgs(ctypes.Structure):
     ]
 
 
+class SolortInt4AppendArgs(ctypes.Structure):
+    """Mirror of ``SolortInt4AppendArgs`` in ``include/solort_attn.h``."""
+
+    _fields_ = [
+        ("qkv", c_vp), ("qkv_stride_token", c_i64),
+        ("num_tokens", c_i32), ("num_qo_heads", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("q_norm_weight", c_vp), ("k_norm_weight", c_vp),
+        ("eps", c_f32),
+        ("cos", c_vp), ("sin", c_vp), ("rope_stride", c_i64), ("rope_rows", c_i32),
+        ("positions", c_vp), ("slots", c_vp),
+        ("q_out", c_vp), ("q_out_stride_token", c_i64), ("q_out_stride_head", c_i64),
+        ("kv_pages", c_vp), ("kv_stride_page", c_i64), ("kv_stride_head", c_i64),
+        ("page_size", c_i32), ("num_pages", c_i32),
+    ]
+
+
+class SolortInt4StoreArgs(ctypes.Structure):
+    """Mirror of ``SolortInt4StoreArgs`` in ``include/solort_attn.h``."""
+
+    _fields_ = [
+        ("key", c_vp), ("value", c_vp),
+        ("key_stride_token", c_i64), ("key_stride_head", c_i64),
+        ("value_stride_token", c_i64), ("value_stride_head", c_i64),
+        ("num_tokens", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32),
+        ("slots", c_vp),
+        ("kv_pages", c_vp), ("kv_stride_page", c_i64), ("kv_stride_head", c_i64),
+        ("page_size", c_i32), ("num_pages", c_i32),
+    ]
+
+
+class SolortInt4LoadArgs(ctypes.Structure):
+    """Mirror of ``SolortInt4LoadArgs`` in ``include/solort_attn.h``."""
+
+    _fields_ = list(SolortInt4StoreArgs._fields_)
+
+
+class SolortInt4DecodeArgs(ctypes.Structure):
+    """Mirror of ``SolortInt4DecodeArgs`` in ``include/solort_attn.h``."""
+
+    _fields_ = [
+        ("q", c_vp),
+        ("q_stride_batch", c_i64), ("q_stride_token", c_i64), ("q_stride_head", c_i64),
+        ("out", c_vp),
+        ("out_stride_batch", c_i64), ("out_stride_token", c_i64), ("out_stride_head", c_i64),
+        ("kv_pages", c_vp), ("kv_stride_page", c_i64), ("kv_stride_head", c_i64),
+        ("page_size", c_i32), ("num_pages", c_i32),
+        ("block_table", c_vp), ("block_table_stride", c_i64),
+        ("q_pos", c_vp), ("q_lens", c_vp),
+        ("batch", c_i32), ("q_len", c_i32), ("num_qo_heads", c_i32), ("num_kv_heads", c_i32),
+        ("head_dim", c_i32),
+        ("max_kv_len", c_i32),
+        ("scale", c_f32),
+        ("num_ctas", c_i32),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+        ("flags", ctypes.c_uint32),
+    ]
+
+
 _LIB: ctypes.CDLL | None = None
 
 
@@ -272,6 +335,13 @@ def _optional_symbols(lib: ctypes.CDLL) -> None:
     lib.solort_attn_gemv.restype = ctypes.c_int
     lib.solort_attn_kv_store.argtypes = [P(SolortKVStoreArgs), c_vp]
     lib.solort_attn_kv_store.restype = ctypes.c_int
+    for name, args in (("qk_norm_rope_append_int4", SolortInt4AppendArgs),
+                       ("kv_store_int4", SolortInt4StoreArgs), ("kv_load_int4", SolortInt4LoadArgs),
+                       ("decode_int4", SolortInt4DecodeArgs)):
+        fn = getattr(lib, "solort_attn_" + name)
+        fn.argtypes, fn.restype = [P(args), c_vp], ctypes.c_int
+    lib.solort_attn_decode_int4_workspace_size.argtypes = [P(SolortInt4DecodeArgs), P(c_sz)]
+    lib.solort_attn_decode_int4_workspace_size.restype = ctypes.c_int
 
 
 class SolortPrefillArgs(ctypes.Structure):

@@ -15,8 +15,9 @@ import math
 
 import torch
 
-from solort_b200 import _calls, _lib
+from solort_b200 import _calls, _calls_int4, _lib
 from solort_b200 import torch_ops  # noqa: F401  (registers torch.ops.solort_attn.*)
+from solort_b200 import torch_ops_int4  # noqa: F401  (the 4-bit KV cache's)
 from solort_b200._calls import (  # noqa: F401  (re-exported for callers of the C-ABI helpers)
     HEAD_DIM, _check_cuda, _decode_args, _ptr, _run_decode, _static_kv, _stream, _stream_at,
     decode_workspace_bytes)
@@ -541,3 +542,120 @@ def kv_store(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
     launch instead of a Python loop over tokens."""
     _OPS.kv_store(key, value, slots, kv_pages)
 
+
+
+# ---- the paged KV cache held in 4 bits ----
+
+def kv_pages_int4(num_pages: int, num_kv_heads: int, page_size: int,
+                  device: torch.device | str = "cuda") -> torch.Tensor:
+    """One layer's arena of the 4-bit paged KV cache, zero-filled: uint8 ``[num_pages, nkv, 160 * P]``
+    for pages of ``P`` tokens (a power of two >= 8). Slots and block tables are those of the bf16 arena
+    ``[num_pages, 2, P, nkv, 128]``; a token and head take 160 bytes instead of 512. Values are held
+    in groups of 32 as ``mid + scale * (code - 7.5)``, within ``scale / 2`` (``include/solort_attn.h``
+    has the layout)."""
+    pages = torch.zeros(num_pages, num_kv_heads, _calls_int4.TOKEN_BYTES * page_size, dtype=torch.uint8,
+                        device=device)
+    _calls_int4.page_size(pages)
+    return pages
+
+
+def kv_store_int4(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
+                  kv_pages: torch.Tensor) -> None:
+    """Hold ``key / value [tokens, nkv, 128]`` (bf16; token / head strides multiples of 8) in 4 bits at
+    ``slots`` (int64 on the device, ``page * P + row``; -1 skips a row) of ``kv_pages``
+    (:func:`kv_pages_int4`; ``torch.ops.solort_attn.kv_store_int4``): the 4-bit :func:`kv_store`."""
+    _OPS.kv_store_int4(key, value, slots, kv_pages)
+
+
+def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tensor | None = None,
+                 value: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values held at ``slots`` as bf16 ``(key, value) [tokens, nkv, 128]``
+    (``torch.ops.solort_attn.kv_load_int4``): a cached prefix for :func:`gqa_prefill`, for one. Rows
+    of slot -1 are not written (undefined in tensors that this call allocates)."""
+    shape = (slots.shape[0], kv_pages.shape[1], HEAD_DIM)
+    if key is None:
+        key = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
+    if value is None:
+        value = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
+    _OPS.kv_load_int4(kv_pages, slots, key, value)
+    return key, value
+
+
+def qk_norm_rope_append_int4(
+    qkv: torch.Tensor,
+    q_norm_weight: torch.Tensor,
+    k_norm_weight: torch.Tensor,
+    eps: float,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    kv_pages: torch.Tensor,
+    *,
+    num_qo_heads: int,
+    num_kv_heads: int,
+    q_out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The attention prologue of a batch into the 4-bit cache, in one launch: QK-RMSNorm + RoPE of
+    ``qkv [t, (nh + 2 nkv) * 128]``, queries to ``q_out [t, nh, 128]``, K / V held at ``slots``.
+
+    ``positions`` and ``slots`` (int64 ``[t]`` on the device) are each token's position in its
+    sequence and its ``page * P + row``: the rows of a prompt, one token of each of many sequences,
+    or any mix. A token of slot -1 (a padded row of a captured batch) is skipped, its ``q_out`` row
+    too. ``cos``/``sin`` as in :func:`qk_norm_rope_append`. Norm and rotation are fp32 with one
+    rounding at the end."""
+    if kv_pages.shape[1] != num_kv_heads:
+        raise RuntimeError(f"kv_pages has {kv_pages.shape[1]} KV heads, not {num_kv_heads}")
+    if q_out is None:
+        q_out = torch.empty(qkv.shape[0], num_qo_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
+    elif q_out.dim() != 3 or q_out.shape[1] != num_qo_heads:
+        raise RuntimeError(f"q_out must be [tokens, {num_qo_heads}, 128]")
+    _OPS.qk_norm_rope_append_int4(qkv, q_norm_weight, k_norm_weight, float(eps), cos, sin, positions,
+                                  slots, kv_pages, q_out)
+    return q_out
+
+
+def decode_int4_workspace_bytes(batch: int, q_len: int, num_qo_heads: int, num_kv_heads: int,
+                                max_kv_len: int, *, num_ctas: int = 0) -> int:
+    """Workspace bytes a :func:`gqa_decode_paged_int4` call with these sizes needs on the current
+    device (0 up to 256 keys; some MiB at most, whatever the batch and the lengths)."""
+    return _calls_int4.decode_workspace_bytes(batch, q_len, num_qo_heads, num_kv_heads, max_kv_len,
+                                              num_ctas)
+
+
+def gqa_decode_paged_int4(
+    q: torch.Tensor,
+    kv_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    q_pos: torch.Tensor,
+    *,
+    max_kv_len: int,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    q_lens: torch.Tensor | None = None,
+    num_ctas: int = 0,
+    stable_prefix: bool = False,
+) -> torch.Tensor:
+    """GQA attention of ``q [B, q_len, nh, 128]`` against one layer of the 4-bit paged cache
+    (``torch.ops.solort_attn.gqa_decode_paged_int4``): :func:`gqa_decode_paged` for ``kv_pages`` of
+    :func:`kv_pages_int4`, for any ``q_len``.
+
+    ``q_pos`` (int64 ``[B]``), ``q_lens``, ``block_table``, ``max_kv_len`` and ``stable_prefix`` as
+    there: row ``i`` sees keys ``0 .. q_pos + i`` below ``max_kv_len``, rows that see none are zero,
+    rows past ``q_lens`` are not written. The keys of all sequences are divided evenly over the GPU,
+    so lengths may differ freely. ``num_ctas`` (0: one resident wave) is for tests. ``out`` and
+    ``workspace`` (:func:`decode_int4_workspace_bytes`) are allocated when not given (pass both to
+    capture the call in a CUDA graph)."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    if workspace is None:
+        _, a = _calls_int4.decode_args(q, kv_pages, block_table, q_pos, out, int(max_kv_len), scale,
+                                       q_lens, int(num_ctas), stable_prefix)
+        need = _calls_int4.decode_workspace_bytes(a.batch, a.q_len, a.num_qo_heads, a.num_kv_heads,
+                                                  a.max_kv_len, a.num_ctas) if q.numel() else 0
+        workspace = (torch.empty(need, dtype=torch.uint8, device=q.device) if need
+                     else _empty_workspace(q.device))
+    _OPS.gqa_decode_paged_int4(q, kv_pages, block_table, q_pos, out, workspace, int(max_kv_len), scale,
+                               q_lens, int(num_ctas), bool(stable_prefix))
+    return out
