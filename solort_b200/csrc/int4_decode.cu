@@ -1,27 +1,33 @@
 // GQA decode / verify attention over the paged 4-bit KV cache (layout and formula: int4.cuh).
 //
 // With keys held as k = mid + scale (c - 7.5) and values likewise, per group g of 32 dims,
-//   q . k       = sum_g scale_g (sum_d q_d c_d - 7.5 sum_d q_d) + mid_g sum_d q_d
-//   sum_t p v_d = sum_t (p scale_g) c_d - 7.5 sum_t (p scale_g) + sum_t p mid_g
-// so the tensor cores multiply the integer codes and the scales are applied to their fp32 results
-// (keys) or to the probabilities (values): the cache is never expanded. A nibble becomes a bf16
-// operand in one and-or: 0x4300 | c is the bf16 number 128 + c exactly, and the 128 joins the 7.5
-// in the two correction terms (both are taken of exactly the bf16 numbers that the products use, so
-// they cancel in the fp32 accumulators). The one rounding on the way is p scale to bf16, the same
-// half step as p's in a bf16 attention, against codes symmetric about zero.
+//   q . k       = sum_g scale_g sum_d q_d c_d + (mid_g - 7.5 scale_g) sum_d q_d
+//   sum_t p v_d = sum_t (p scale_g) c_d + sum_t p (mid_g - 7.5 scale_g)
+// so the tensor cores multiply the codes themselves and the scales are applied to their fp32 results
+// (keys) or to the probabilities (values): the cache is never expanded. The products run in e4m3,
+// because a nibble in a byte IS an e4m3 number: bytes 0..15 are the subnormals and the first binade,
+// the values c 2^-9 exactly. Eight codes become operands with a shift and two ands, half of what a
+// bf16 operand costs, and the e4m3 product takes a quarter of the bf16 one's time per multiply-add
+// (measured: m16n8k32 e4m3 4.6 cycles a scheduler, m16n8k16 bf16 8.8; results exact to fp32).
 //
-// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16, tokens or dims as
-// the 16 rows, query rows as the 8 columns), so that the few query rows of a decode fill an n8 tile;
-// P^T turns into the second product's operand with movmatrix. The rate that the memory asks for
-// (0.28 tokens of a head per ns and SM) leaves 27 warp instructions per token and head; this form
-// needs about 16. tcgen05 would leave them as they are: the work is unpacking codes, which its
-// shared-memory operands would have to be written back for.
+// The other operand is split in two e4m3 numbers, hi and lo, four significant bits each, lo times
+// 16; they are the two columns of one query row. A query row is scaled by a power of two to a
+// maximum in [128, 256): hi + lo / 16 is then its bf16 values exactly down to 2^-13 of the row's maximum,
+// and within 2^-22 of that maximum below. For values it is x = 2^8 p scale sf, with p relative to the
+// row's running maximum and sf the power of two that brings the group's scales below 1: hi + lo / 16 is
+// within 2^-9 x (2^-8 next to a power of two: bf16's half step), and again within 2^-22 of the maximum
+// for x below 2^-13 of it. The codes are centred with the sum of the same numbers (a product with
+// ones), O = sum x c - 7.5 sum x + sum p mid, so that their rounding weighs |v - mid| and not c.
 //
-// Work split: the cache's 16-token tiles, over all sequences, KV heads and blocks of query rows, are
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k32, tokens or dims as the 16
+// rows), so that four query rows fill an n8 tile; P^T turns into the second product's operand with
+// movmatrix, two tokens' bytes to an element.
+//
+// Work split: the cache's 32-token tiles, over all sequences, KV heads and blocks of query rows, are
 // one list, and CTA c of n takes the tiles [T c / n, T (c + 1) / n): sequences of any lengths load
 // every SM alike, and the workspace is two partials per CTA whatever the batch. A CTA's eight warps
-// take its tiles in turn, each warp with a ring of kDepth tiles of its own (one bulk copy of 2560
-// contiguous bytes a tile, an mbarrier each), so warps meet only at the end of a (sequence, head)
+// take its tiles in turn, each warp with a ring of kDepth tiles of its own (5120 bytes a tile, one bulk
+// copy for each page that it touches, an mbarrier), so warps meet only at the end of a (sequence, head)
 // segment. A segment that is a whole (sequence, head) writes its final rows; parts meet in
 // merge_kernel. Lengths are read on the device, and merge_kernel repeats the same division.
 //
@@ -39,28 +45,32 @@ __device__ unsigned g_int4_decode_status;
 
 namespace i4 {
 
-constexpr int kTile = 16;                          // tokens of a tile: two blocks
-constexpr int kTileBytes = 2 * kBlockBytes;        // 2560
-constexpr int kDepth = 4;                          // tiles in flight per warp
-constexpr int kWarps = 8;
+constexpr int kTile = 32;                     // tokens of a tile: four blocks
+constexpr int kTileBytes = 4 * kBlockBytes;   // 5120
+constexpr int kDepth = 3;                     // tiles of a warp in shared memory
+constexpr int kWarps = 6;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinTiles = kWarps;                  // tiles per CTA at least: one per warp
-constexpr int kDirectTiles = 2 * kWarps;           // up to this many tiles a (sequence, head) is one CTA
-constexpr float kShift = 135.5f;                   // 128 of the bf16 codes and 7.5 of the formula
-// A row's running maximum is raised only when a score passes it by 2^8: p stays below 2^8, far
-// inside bf16 and fp32, and the accumulators are rescaled a few times per split instead of always.
-constexpr float kLazy = 8.f;
+constexpr int kUnitCost = 2;                  // tiles' worth of set-up of a (sequence, head, row block)
+constexpr int kDirectTiles = 2 * kWarps;      // up to this many tiles a (sequence, head) is one CTA
+// A row's running maximum is raised only when a score passes it by 2^kLazy; p is 2^kPShift there, so
+// that x stays below 2^15, inside f16.
+constexpr float kLazy = 7.f;
+constexpr float kPShift = 15.f - kLazy;
+constexpr float kCodeUnit = 512.f;         // a key code's e4m3 value is c / 512
+constexpr float kValueUnit = 16777216.f;   // a value code's f16 value is c 2^-24, or 16 c 2^-24
 
-template <int NT>  // n8 tiles of query rows
+template <int NT>  // n8 tiles: four query rows each
 struct Cfg {
-  static constexpr int kRows = 8 * NT;
+  static constexpr int kRows = 4 * NT;
   static constexpr int kRing = kWarps * kDepth * kTileBytes;
   static constexpr int kRed = kWarps * kRows * kHD * 4;
+  static_assert(kRows * kHD * 4 <= kDepth * kTileBytes, "a part fits a ring");
   static constexpr int kOffRed = kRing;
-  static constexpr int kOffMl = kOffRed + kRed;                  // [warp][row] (max, sum)
-  static constexpr int kOffBar = kOffMl + kWarps * kRows * 8;    // [warp][depth]
-  static constexpr int kOffFlag = kOffBar + kWarps * kDepth * 8;
-  static constexpr int kSmem = kOffFlag + 16;
+  static constexpr int kOffMl = kOffRed + kRed;
+  static constexpr int kOffEdge = kOffMl + 2 * kWarps * kRows * 8;
+  static constexpr int kOffRange = kOffEdge + 2 * kWarps * 4;
+  static constexpr int kOffPlaces = (kOffRange + (kWarps + 1) * 12 + 15) / 16 * 16;  // [warp][32 tiles][4]
+  static constexpr int kSmem = kOffPlaces + kWarps * 32 * 32;
   static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
 };
 static_assert(Cfg<1>::kSmem <= 115712, "two CTAs per SM");
@@ -91,6 +101,7 @@ struct Seq {  // one sequence's share of the list
   int kv_end, rows, rb, tiles;
   __device__ __forceinline__ int units(int nkv) const { return nkv * rb; }
   __device__ __forceinline__ int total(int nkv) const { return nkv * rb * tiles; }
+  __device__ __forceinline__ int cost(int nkv) const { return tiles ? nkv * rb * (tiles + kUnitCost) : 0; }
 };
 
 template <int NT>
@@ -108,59 +119,48 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int b) {
   return s;
 }
 
-__device__ __forceinline__ int warp_inclusive(int v) {
+// Prefix sums over the sequences, 32 at a time: lane i has sequence first + i.
+struct Prefix {
+  int cost, tiles, unit_tiles;  // of this lane's sequence: in all, and of one unit
+  int cost_incl, tiles_incl;    // sums from `first` on
+  int cost_run, tiles_run;      // before `first`
+};
+template <int NT>
+__device__ __forceinline__ void load_prefix(const Params& p, Prefix& f, int first) {
+  const int lane = threadIdx.x & 31;
+  f.cost_run = first ? f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl, 31) : 0;
+  f.tiles_run = first ? f.tiles_run + __shfl_sync(0xffffffffu, f.tiles_incl, 31) : 0;
+  f.cost = f.tiles = f.unit_tiles = 0;
+  if (first + lane < p.batch) {
+    const Seq s = load_seq<NT>(p, first + lane);
+    f.cost = s.cost(p.nkv);
+    f.tiles = s.total(p.nkv);
+    f.unit_tiles = s.tiles;
+  }
+  f.cost_incl = f.cost;
+  f.tiles_incl = f.tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) >= o) v += u;
+    const int u = __shfl_up_sync(0xffffffffu, f.cost_incl, o), v = __shfl_up_sync(0xffffffffu, f.tiles_incl, o);
+    if (lane >= o) f.cost_incl += u, f.tiles_incl += v;
   }
-  return v;
 }
 
-// All tiles of the list; and the tiles before sequence `b` (with the whole warp).
-template <int NT>
-__device__ __forceinline__ int list_total(const Params& p, int b, int* before) {
-  const int lane = threadIdx.x & 31;
-  int run = 0;
-  for (int c = 0; c < p.batch; c += 32) {
-    const int v = c + lane < p.batch ? load_seq<NT>(p, c + lane).total(p.nkv) : 0;
-    const int incl = warp_inclusive(v);
-    if (b >= c && b < c + 32) *before = run + __shfl_sync(0xffffffffu, incl - v, b - c);
-    run += __shfl_sync(0xffffffffu, incl, 31);
+// CTAs at work on a list of that cost, and its division between workers: the first cost % n of n have
+// one position more than the others.
+struct Division {
+  int n, each, more;
+  __device__ __forceinline__ Division(int cost, int ctas) {
+    n = max(1, min(ctas, (cost + kWarps - 1) / kWarps)) * kWarps;
+    each = cost / n;
+    more = cost - each * n;
   }
-  return run;
-}
-
-// The sequence that holds tile x < total, and the tiles before it.
-template <int NT>
-__device__ __forceinline__ int find_seq(const Params& p, int x, int* before) {
-  const int lane = threadIdx.x & 31;
-  int run = 0;
-  for (int c = 0; c < p.batch; c += 32) {
-    const int v = c + lane < p.batch ? load_seq<NT>(p, c + lane).total(p.nkv) : 0;
-    const int incl = warp_inclusive(v);
-    const unsigned past = __ballot_sync(0xffffffffu, x < run + incl);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      *before = run + __shfl_sync(0xffffffffu, incl - v, l);
-      return c + l;
-    }
-    run += __shfl_sync(0xffffffffu, incl, 31);
+  __device__ __forceinline__ int first(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int worker(int x) const {
+    const int split = more * (each + 1);
+    return x < split ? x / (each + 1) : more + (x - split) / each;
   }
-  *before = run;
-  return p.batch;
-}
-
-// CTAs at work on a list of `total` tiles, and the first tile of CTA c.
-__device__ __forceinline__ int active_ctas(int total, int ctas) {
-  return max(1, min(ctas, (total + kMinTiles - 1) / kMinTiles));
-}
-__device__ __forceinline__ int first_tile(int total, int n, int c) {
-  return static_cast<int>(static_cast<long long>(total) * c / n);
-}
-__device__ __forceinline__ int cta_of(int total, int n, int x) {
-  return static_cast<int>(((x + 1ll) * n - 1) / total);
-}
+};
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -172,9 +172,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {  // 128 + nibble, low and high half
-  return (w & 0x000f000fu) | 0x43004300u;
-}
+constexpr uint32_t kNibbles = 0x0f0f0f0fu;
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -185,137 +183,302 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {  // all but the last N groups of this thread have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// d = a b + c, m16n8k32 e4m3.
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         float c0, float c1, float c2, float c3) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Pairs of fp32 (the packed instructions take half the issue slots).
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 dup(float a) { return pair(a, a); }
+
+// d += a b, m16n8k16 f16.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
 }
 
-// One warp's state over a segment.
+// One warp's state over a segment. This lane's query row of n8 tile nt is row 4 nt + lane % 4.
 template <int NT>
 struct Acc {
-  float o[NT][4][2][4];  // [group][m16 tile]: dims 32g + 4 (lane / 4) + 2h, + 1; rows 2 (lane % 4), + 1
-  float ps[NT][2][4];    // sums of the bf16 p scale: groups 2i (c0, c1) and 2i + 1 (c2, c3)
-  float pm[NT][4][2];    // this lane's tokens' sum of p mid
-  float l[NT][2], m[NT][2];
+  static constexpr int kCols = NT > 1 ? NT / 2 : 1;  // n8 tiles of the second product
+  // [tile][group][m16 tile h]: c0, c1 dim 32 g + 4 (lane / 4) + 2 h, c2, c3 the dim after. The columns
+  // are two rows (nt = 2 tile, 2 tile + 1), or with one row a lane that row for the two groups of a
+  // pair, of which the one is the group's own and the other is waste.
+  float o[kCols][4][2][4];
+  // Sums of x: [tile][group pair], columns of the even group in c0, c1 and of the odd in c2, c3; with
+  // one row a lane [0][0], of the pair 0 and 1.
+  float xs[kCols][NT > 1 ? 2 : 1][4];
+  f2 pm[NT][2];   // this lane's tokens' sum of p mid, a group pair each
+  float l[NT];    // and of p
+  float off[NT];  // p = 2^(score - off)
+  float top[NT];  // scores above it raise the maximum
+  f2 sf[2];       // per group pair
 };
 
-// One tile of 16 tokens for the segment's rows. MASKED: some row does not see some token.
-template <int NT, bool MASKED>
-__device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT][4][4],
-                                          const float (&qs)[NT][4][2], Acc<NT>& A, float scale_log2,
-                                          const int (&lim)[NT][2], int tok0, bool ok0, bool ok1) {
+// One tile of 32 tokens for the segment's rows; this lane's tokens are tok0 + 8 i + lane / 4 of block
+// i. `masked`: some row does not see some token; `there` has a bit for each block that was loaded.
+template <int NT>
+__device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT][4][2],
+                                          const uint32_t (&qm)[NT][2], Acc<NT>& A, const float (&fr)[NT],
+                                          bool masked, const int (&lim)[NT], int tok0, unsigned there) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float s[NT][4];
-  {
-    const uint4 k0 = lds128(base + 64 * g + 16 * t), k1 = lds128(base + kBlockBytes + 64 * g + 16 * t);
-    const uint4 m0 = lds128(base + kOffKScale + 16 * g);
-    const uint4 m1 = lds128(base + kBlockBytes + kOffKScale + 16 * g);
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) {
+    const uint32_t b0 = base + 2 * mt * kBlockBytes, b1 = b0 + kBlockBytes;
+    const uint4 k0 = lds128(b0 + 64 * g + 16 * t), k1 = lds128(b1 + 64 * g + 16 * t);
+    const uint4 m0 = lds128(b0 + kOffKScale + 16 * g), m1 = lds128(b1 + kOffKScale + 16 * g);
+    f2 acc[NT];
+    {
+      // sum_g (mid_g - 7.5 scale_g) sum_d q_d, a product itself: k = mids, mids, scales, scales of the four
+      // groups against the sums of q, their low parts, and both times -7.5.
+      const uint2 n0 = lds64(b0 + kOffKScale + 16 * g + 8 * (t & 1)), n1 = lds64(b1 + kOffKScale + 16 * g + 8 * (t & 1));
+      const uint32_t a[4] = {__byte_perm(n0.x, n0.y, 0x7632), __byte_perm(n1.x, n1.y, 0x7632),
+                             __byte_perm(n0.x, n0.y, 0x5410), __byte_perm(n1.x, n1.y, 0x5410)};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_bf16_16816(c, a, qm[nt][0], qm[nt][1]);
+        acc[nt] = pair(c[0], c[2]);
+      }
+    }
 #pragma unroll
     for (int grp = 0; grp < 4; ++grp) {
       const uint32_t w0 = word(k0, grp), w1 = word(k1, grp);
-      const uint32_t a0[4] = {codes_bf16(w0), codes_bf16(w1), codes_bf16(w0 >> 4), codes_bf16(w1 >> 4)};
-      const uint32_t a1[4] = {codes_bf16(w0 >> 8), codes_bf16(w1 >> 8), codes_bf16(w0 >> 12),
-                              codes_bf16(w1 >> 12)};
-      const float s0 = lo_bf16(word(m0, grp)), d0 = hi_bf16(word(m0, grp));
-      const float s1 = lo_bf16(word(m1, grp)), d1 = hi_bf16(word(m1, grp));
+      const uint32_t a[4] = {w0 & kNibbles, w1 & kNibbles, (w0 >> 4) & kNibbles, (w1 >> 4) & kNibbles};
+      const f2 sc = pair(lo_bf16(word(m0, grp)), lo_bf16(word(m1, grp)));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float q0 = qs[nt][grp][0], q1 = qs[nt][grp][1];
-        float c[4] = {-kShift * q0, -kShift * q1, -kShift * q0, -kShift * q1};
-        mma_bf16_16816(c, a0, qf[nt][grp][0], qf[nt][grp][1]);
-        mma_bf16_16816(c, a1, qf[nt][grp][2], qf[nt][grp][3]);
-        if (grp == 0) {
-          s[nt][0] = s0 * c[0] + d0 * q0;
-          s[nt][1] = s0 * c[1] + d0 * q1;
-          s[nt][2] = s1 * c[2] + d1 * q0;
-          s[nt][3] = s1 * c[3] + d1 * q1;
-        } else {
-          s[nt][0] += s0 * c[0] + d0 * q0;
-          s[nt][1] += s0 * c[1] + d0 * q1;
-          s[nt][2] += s1 * c[2] + d1 * q0;
-          s[nt][3] += s1 * c[3] + d1 * q1;
-        }
+        float c[4];
+        mma_e4m3(c, a, qf[nt][grp][0], qf[nt][grp][1], 0.f, 0.f, 0.f, 0.f);
+        acc[nt] = fma2(sc, pair(fmaf(c[1], 0.0625f, c[0]), fmaf(c[3], 0.0625f, c[2])), acc[nt]);
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 x = both(mul2(acc[nt], dup(fr[nt])));
+      s[nt][2 * mt] = x.x, s[nt][2 * mt + 1] = x.y;
+    }
   }
-  bool vis[NT][4];
+  uint4 meta[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) meta[i] = lds128(base + i * kBlockBytes + kOffVScale + 16 * g);
+  if (__builtin_expect(masked, 0)) {
+    // A token that a row does not see adds nothing, whatever its scale and mid are: they count as 0
+    // where no row of the lane sees it, and where some do, a NaN goes into those rows' scores.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bool any = false, all = true;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const bool vis = (there >> i & 1u) && tok0 + 8 * i + g <= lim[nt];
+        if (!vis) s[nt][i] = -INFINITY;
+        any |= vis;
+        all &= vis;
+      }
+      bool drop = !any;
+      if (NT > 1 && any && !all) {
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp)
+          drop |= isnan(lo_bf16(word(meta[i], grp))) || isnan(hi_bf16(word(meta[i], grp)));
+        if (drop)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (tok0 + 8 * i + g <= lim[nt]) s[nt][i] = NAN;
+      }
+      if (drop) meta[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
   bool raise = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
+    raise |= fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3])) > A.top[nt];
+  f2 sc[4][2];  // [token][group pair] scale * sf, at most 1
+  float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[nt][i] *= scale_log2;
-      if (MASKED) {
-        vis[nt][i] = (i < 2 ? ok0 && tok0 + g <= lim[nt][i & 1] : ok1 && tok0 + 8 + g <= lim[nt][i & 1]);
-        if (!vis[nt][i]) s[nt][i] = -INFINITY;
-      }
-      raise |= s[nt][i] > A.m[nt][i & 1] + kLazy;
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      sc[i][q] = mul2(pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1))), A.sf[q]);
+      const float2 v = both(sc[i][q]);
+      most = fmaxf(most, fmaxf(v.x, v.y));
     }
-  if (__any_sync(0xffffffffu, raise)) {
+  raise |= most > 1.f;
+  if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+    if (__any_sync(0xffffffffu, most > 1.f)) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int grp = 0; grp < 4; ++grp) {
+        const int q = grp >> 1, e = grp & 1;
+        float mx = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, lo_bf16(word(meta[i], grp)));
 #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        mx = fmaxf(mx, A.m[nt][e]);
-        const float f = A.m[nt][e] == -INFINITY ? 0.f : ex2(A.m[nt][e] - mx);
-        A.m[nt][e] = mx;
-        A.l[nt][e] *= f;
+        for (int o = 1; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float2 old = both(A.sf[q]);
+        const float was = e ? old.y : old.x;
+        if (mx * was > 1.f) {  // the power of two that brings mx into [0.5, 1)
+          const int top = 253 - static_cast<int>(__float_as_uint(mx) >> 23);
+          const float sf = __uint_as_float(static_cast<uint32_t>(max(top, 1)) << 23), f = sf / was;
+          A.sf[q] = e ? pair(old.x, sf) : pair(sf, old.y);
 #pragma unroll
-        for (int grp = 0; grp < 4; ++grp) {
-          A.pm[nt][grp][e] *= f;
-          A.ps[nt][grp >> 1][(grp & 1) * 2 + e] *= f;
+          for (int c = 0; c < Acc<NT>::kCols; ++c) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            A.o[nt][grp][h][e] *= f;
-            A.o[nt][grp][h][2 + e] *= f;
+            for (int i = 0; i < 4; ++i) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
+            if (NT > 1)
+              A.xs[c][q & (NT > 1)][2 * e] *= f, A.xs[c][q & (NT > 1)][2 * e + 1] *= f;
+            else
+              A.xs[c][0][2 * q + e] *= f;
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          sc[i][q] = mul2(pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1))), A.sf[q]);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float mx = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (mx > A.top[nt]) {
+        const float off = mx - kPShift, f = A.top[nt] == -INFINITY ? 0.f : ex2(A.off[nt] - off);
+        A.off[nt] = off;
+        A.top[nt] = mx + kLazy;
+        A.l[nt] *= f;
+        A.pm[nt][0] = mul2(A.pm[nt][0], dup(f));
+        A.pm[nt][1] = mul2(A.pm[nt][1], dup(f));
+        const int c = nt / 2, e = nt & 1;
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (NT == 1 || (i & 1) == e) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (NT == 1)
+            A.xs[0][0][i] *= f;
+          else if ((i & 1) == e)
+            A.xs[c][0][i] *= f, A.xs[c][NT > 1][i] *= f;
+      }
+    }
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float m = A.m[nt][i & 1];
-      s[nt][i] = ex2(s[nt][i] - (MASKED && m == -INFINITY ? 0.f : m));
-      A.l[nt][i & 1] += s[nt][i];
+      s[nt][i] = ex2(s[nt][i] - A.off[nt]);
+      A.l[nt] += s[nt][i];
     }
 
-  const uint32_t va = base + kOffV + 128 * t + 16 * (g ^ (2 * t));
-  const uint4 v0 = lds128(va), v1 = lds128(va + kBlockBytes);
-  const uint4 m0 = lds128(base + kOffVScale + 16 * g);
-  const uint4 m1 = lds128(base + kBlockBytes + kOffVScale + 16 * g);
-  constexpr uint32_t kOnes = 0x3f803f80u;
+  uint4 v[4];
 #pragma unroll
-  for (int grp = 0; grp < 4; ++grp) {
-    const float s0 = lo_bf16(word(m0, grp)), d0 = hi_bf16(word(m0, grp));
-    const float s1 = lo_bf16(word(m1, grp)), d1 = hi_bf16(word(m1, grp));
-    const uint32_t w0 = word(v0, grp), w1 = word(v1, grp);
-    const uint32_t a0[4] = {codes_bf16(w0), codes_bf16(w0 >> 4), codes_bf16(w1), codes_bf16(w1 >> 4)};
-    const uint32_t a1[4] = {codes_bf16(w0 >> 8), codes_bf16(w0 >> 12), codes_bf16(w1 >> 8),
-                            codes_bf16(w1 >> 12)};
-    const uint32_t ones[4] = {grp & 1 ? 0u : kOnes, grp & 1 ? kOnes : 0u, grp & 1 ? 0u : kOnes,
-                              grp & 1 ? kOnes : 0u};
+  for (int i = 0; i < 4; ++i) v[i] = lds128(base + i * kBlockBytes + kOffV + 128 * t + 16 * (g ^ (2 * t)));
+  constexpr uint32_t kOnes = 0x3c003c00u, kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float x[4];
+  for (int q = 0; q < 2; ++q) {
+    f2 x[NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // A token that a row does not see adds nothing, whatever its scale and mid are.
-        const float sc = i < 2 ? s0 : s1, md = i < 2 ? d0 : d1;
-        x[i] = MASKED && !vis[nt][i] ? 0.f : s[nt][i] * sc;
-        A.pm[nt][grp][i & 1] += MASKED && !vis[nt][i] ? 0.f : s[nt][i] * md;
+    for (int i = 0; i < 4; ++i) {
+      const f2 mid = pair(hi_bf16(word(meta[i], 2 * q)), hi_bf16(word(meta[i], 2 * q + 1)));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        x[nt][i] = mul2(dup(s[nt][i]), sc[i][q]);
+        A.pm[nt][q] = fma2(dup(s[nt][i]), mid, A.pm[nt][q]);
       }
-      const uint32_t b0 = transpose8x8(pack_bf16x2(x[0], x[1]));
-      const uint32_t b1 = transpose8x8(pack_bf16x2(x[2], x[3]));
-      mma_bf16_16816(A.o[nt][grp][0], a0, b0, b1);
-      mma_bf16_16816(A.o[nt][grp][1], a1, b0, b1);
-      mma_bf16_16816(A.ps[nt][grp >> 1], ones, b0, b1);
+    }
+    uint32_t bb[2][Acc<NT>::kCols][4];  // [group of the pair][tile][block]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (NT == 1) {
+        const float2 x0 = both(x[0][i]);
+        bb[0][0][i] = bb[1][0][i] = transpose8x8(pack_f16x2(x0.x, x0.y));
+      } else {
+#pragma unroll
+        for (int c = 0; c < Acc<NT>::kCols; ++c) {
+          const float2 x0 = both(x[2 * c][i]), x1 = both(x[2 * c + (NT > 1)][i]);
+          bb[0][c][i] = transpose8x8(pack_f16x2(x0.x, x1.x));
+          bb[1][c][i] = transpose8x8(pack_f16x2(x0.y, x1.y));
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int grp = 2 * q + e;
+      const uint32_t lo_rows = (NT > 1 ? e : q) ? 0u : kOnes, hi_rows = (NT > 1 ? e : q) ? kOnes : 0u;
+      const uint32_t ones[4] = {lo_rows, hi_rows, lo_rows, hi_rows};
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {  // tokens of blocks k, k + 1
+        const uint32_t w0 = word(v[k], grp), w1 = word(v[k + 1], grp), y0 = w0 >> 8, y1 = w1 >> 8;
+        const uint32_t a0[4] = {w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh};
+        const uint32_t a1[4] = {y0 & kLow, y0 & kHigh, y1 & kLow, y1 & kHigh};
+#pragma unroll
+        for (int c = 0; c < Acc<NT>::kCols; ++c) {
+          mma_f16(A.o[c][grp][0], a0, bb[e][c][k], bb[e][c][k + 1]);
+          mma_f16(A.o[c][grp][1], a1, bb[e][c][k], bb[e][c][k + 1]);
+          if (NT > 1)
+            mma_f16(A.xs[c][q & (NT > 1)], ones, bb[e][c][k], bb[e][c][k + 1]);
+          else if (e == 0)
+            mma_f16(A.xs[c][0], ones, bb[e][c][k], bb[e][c][k + 1]);
+        }
+      }
     }
   }
 }
@@ -328,275 +491,376 @@ __device__ __forceinline__ void write_row4(const Params& p, int b, int kvh, int 
   *reinterpret_cast<uint2*>(p.out + b * p.o_sb + i * p.o_st + h * p.o_sh + c) = pk;
 }
 
+// This lane's chunk of its row of n8 tile nt: dims 32 grp + 4 (lane / 4) .. + 3.
+template <int NT>
+__device__ __forceinline__ float4 chunk_of(const Acc<NT>& A, int nt, int grp, float pm) {
+  const float2 sf = both(A.sf[grp >> 1]);
+  // 1 / sf, a power of two
+  const float inv = __uint_as_float((254u << 23) - __float_as_uint(grp & 1 ? sf.y : sf.x));
+  const int c = nt / 2, e = NT > 1 ? nt & 1 : grp & 1;
+  const float sum = NT > 1 ? A.xs[c][(grp >> 1) & (NT > 1)][(grp & 1) * 2 + e] : A.xs[0][0][grp];
+  const float add = pm - 7.5f * inv * sum, unit = kValueUnit * inv, unit16 = unit * 0.0625f;
+  const float(&a0)[4] = A.o[c][grp][0];
+  const float(&a1)[4] = A.o[c][grp][1];
+  return make_float4(fmaf(unit, a0[e], add), fmaf(unit16, a0[2 + e], add), fmaf(unit, a1[e], add),
+                     fmaf(unit16, a1[2 + e], add));
+}
+
+// A warp's tiles of the list: from x0 on, the sequence of the first and the tiles before that. Entry
+// kWarps is the end of the CTA's.
+struct Range {
+  int x0, seq, base;
+};
+
 template <int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
   using C = Cfg<NT>;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + C::kOffRed);
-  float2* ml = reinterpret_cast<float2*>(smem + C::kOffMl);
-  volatile int* failed = reinterpret_cast<volatile int*>(smem + C::kOffFlag);
+  // What a warp leaves of a unit that it shares with other warps: its first unit's (begun before the
+  // warp's range) in `red`, and its last's (begun in it, going on behind it) where its ring was.
+  float2* ml = reinterpret_cast<float2*>(smem + C::kOffMl);   // [2 warp + which][row]
+  int* edge = reinterpret_cast<int*>(smem + C::kOffEdge);     // [2 warp + which]: the unit's first tile, or -1
+  Range* range = reinterpret_cast<Range*>(smem + C::kOffRange);
+  auto part_row = [&](int which, int row) {
+    return reinterpret_cast<float*>(smem + (which & 1 ? (which >> 1) * kDepth * kTileBytes
+                                                      : C::kOffRed + (which >> 1) * C::kRows * kHD * 4)) + row * kHD;
+  };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + warp * kDepth;
   const uint32_t ring = smem_u32(smem) + warp * kDepth * kTileBytes;
+  // Where the blocks of the warp's next tiles are: an address each, with its count of blocks in the
+  // low bits. Pages of 16 tokens and more: two of two blocks per tile; of 8: four.
+  const uint32_t places = smem_u32(smem) + C::kOffPlaces + warp * 32 * 32;
 
   pdl_launch_dependents();
-  if (lane == 0) {
-    for (int i = 0; i < kDepth; ++i) mbar_init(&bar[i], 1);
-    fence_mbarrier_init();
-  }
-  if (tid == 0) *failed = 0;
-  __syncthreads();
+  if (lane == 0) edge[2 * warp] = edge[2 * warp + 1] = -1;
   const bool early = p.stable_prefix != 0;
   if (!early) pdl_wait();
-
-  // This CTA's tiles [x0, x1) of the list, and the sequence of the first.
-  int x0, x1, b, base;
-  if (p.direct) {
-    b = blockIdx.y;
-    base = 0;
-    const Seq s = load_seq<NT>(p, b);
-    const int unit = blockIdx.x;
-    if (unit >= s.units(p.nkv) || s.tiles == 0) {
-      pdl_wait();
-      const int kvh = s.rb ? unit / s.rb : 0, r0 = s.rb ? (unit % s.rb) * C::kRows : 0;
-      if (unit < s.units(p.nkv))  // rows that see no key
-        for (int i = tid; i < min(C::kRows, s.rows - r0) * (kHD / 4); i += kThreads)
-          write_row4(p, b, kvh, r0 + i / (kHD / 4), (i % (kHD / 4)) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-      return;
+  if (warp == 0) {
+    Range r = {0, 0, 0};
+    if (p.direct) {
+      const Seq s = load_seq<NT>(p, blockIdx.y);
+      r.seq = blockIdx.y;
+      const int unit = blockIdx.x;
+      if (unit < s.units(p.nkv)) r.x0 = unit * s.tiles + s.tiles * min(lane, kWarps) / kWarps;
+    } else {
+      Prefix f;
+      for (int c = 0; c < p.batch; c += 32) load_prefix<NT>(p, f, c);
+      const int cost = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl, 31);
+      const Division d(cost, p.ctas);
+      const int X = d.first(min(static_cast<int>(blockIdx.x) * kWarps + min(lane, kWarps), d.n));
+      r.x0 = f.tiles_run + __shfl_sync(0xffffffffu, f.tiles_incl, 31);  // the end of the list
+      r.seq = p.batch;
+      bool found = false;
+      for (int c = 0; c < p.batch; c += 32) {
+        if (p.batch > 32) load_prefix<NT>(p, f, c);
+        const int y = X - f.cost_run;
+        int l = 0;  // the first sequence of the 32 that ends behind X
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1)
+          if (y >= __shfl_sync(0xffffffffu, f.cost_incl, l + step - 1)) l += step;
+        const int end = __shfl_sync(0xffffffffu, f.cost_incl, l);
+        const int in_seq = y - end + __shfl_sync(0xffffffffu, f.cost, l);
+        const int before = f.tiles_run + __shfl_sync(0xffffffffu, f.tiles_incl - f.tiles, l);
+        const int tiles = __shfl_sync(0xffffffffu, f.unit_tiles, l);
+        if (!found && y < end) {
+          found = true;
+          const int unit = in_seq / (tiles + kUnitCost);
+          r.seq = c + l;
+          r.base = before;
+          r.x0 = before + unit * tiles + max(0, in_seq - unit * (tiles + kUnitCost) - kUnitCost);
+        }
+      }
     }
-    x0 = unit * s.tiles;
-    x1 = x0 + s.tiles;
-  } else {
-    int unused = 0;
-    const int total = list_total<NT>(p, -1, &unused);
-    const int n = active_ctas(total, p.ctas);
-    if (total == 0 || static_cast<int>(blockIdx.x) >= n) {
-      pdl_wait();
-      return;
-    }
-    x0 = first_tile(total, n, blockIdx.x);
-    x1 = first_tile(total, n, blockIdx.x + 1);
-    b = find_seq<NT>(p, x0, &base);
+    if (lane <= kWarps) range[lane] = r;
   }
+  __syncthreads();
+  const int x0 = range[warp].x0, x1 = range[warp + 1].x0;
+  int b = range[warp].seq, base = range[warp].base;
 
-  // ---- the copies: lane i of the warp holds the addresses of the warp's tile 32 k + i ----
-  const int mine = x1 - x0 > warp ? (x1 - x0 - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
-  int ib = b, ibase = base;                        // sequence of this lane's tile
-  const uint8_t *src0 = nullptr, *src1 = nullptr;  // its blocks; nullptr: none, or not in the arena
-  bool stable = false;
-  unsigned none0 = 0, none1 = 0;  // lanes whose first / second block is not there
-  auto resolve = [&](int k) {     // tiles k .. k + 31
-    src0 = src1 = nullptr;
-    stable = false;
-    const int x = x0 + warp + (k + lane) * kWarps;
-    if (k + lane < mine) {
-      Seq s = load_seq<NT>(p, ib);
-      while (x >= ibase + s.total(p.nkv)) {
-        ibase += s.total(p.nkv);
-        s = load_seq<NT>(p, ++ib);
+  // ---- the copies ----
+  const bool by_block = p.page_size == kBlockTokens;
+  int ib = b, ibase = base;  // sequence of this lane's tile of the batch
+  unsigned absent = 0;       // tiles of the batch of which a block should be there and is not
+  unsigned moving = 0;       // tiles of the batch that a kernel before this one may still be writing
+  unsigned gone = 0;         // four bits per ring slot: blocks that should be there and are not
+  auto resolve = [&](int first) {  // the places of tiles first .. first + 31, a lane each
+    bool lost = false, change = false;
+    const int y = first + lane;
+    unsigned long long at[4] = {0, 0, 0, 0};
+    if (y < x1) {
+      Seq is = load_seq<NT>(p, ib);
+      while (y >= ibase + is.total(p.nkv)) {
+        ibase += is.total(p.nkv);
+        is = load_seq<NT>(p, ++ib);
       }
-      const int unit = (x - ibase) / s.tiles, tok = (x - ibase - unit * s.tiles) * kTile;
-      const int head = unit / s.rb;
-      const int32_t* bt = p.block_table + ib * p.bt_stride;
-      const int pg0 = bt[tok >> p.page_shift];
-      int pg1 = pg0;
-      const bool two = s.kv_end - tok > kBlockTokens;
-      if (two && p.page_size == kBlockTokens) pg1 = bt[(tok >> p.page_shift) + 1];
-      const int row = tok & (p.page_size - 1);
-      if (pg0 >= 0 && pg0 < p.num_pages)
-        src0 = p.pages + block_offset(pg0, row, head, p.page_stride, p.head_stride);
-      if (two && pg1 >= 0 && pg1 < p.num_pages)
-        src1 = p.page_size == kBlockTokens
-                   ? p.pages + block_offset(pg1, 0, head, p.page_stride, p.head_stride)
-                   : src0 + kBlockBytes;
-      if (!src0 || (two && !src1)) atomicOr(&g_int4_decode_status, kDevErrPage);
-      stable = tok + kTile <= s.qpos;
+      const int unit = (y - ibase) / is.tiles, head = unit / is.rb;
+      const int tok0 = (y - ibase - unit * is.tiles) * kTile;
+      const int step = by_block ? kBlockTokens : 2 * kBlockTokens;
+      change = tok0 + kTile > is.qpos;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int tok = tok0 + j * step;
+        if (tok >= is.kv_end || tok >= tok0 + kTile) continue;
+        const int page = p.block_table[ib * p.bt_stride + (tok >> p.page_shift)];
+        if (page < 0 || page >= p.num_pages) {
+          at[j] = 8;
+          lost = true;
+        } else {
+          at[j] = reinterpret_cast<unsigned long long>(
+                      p.pages + block_offset(page, tok & (p.page_size - 1), head, p.page_stride, p.head_stride)) +
+                  min(step, is.kv_end - tok + kBlockTokens - 1) / kBlockTokens;
+        }
+      }
+      if (lost) atomicOr(&g_int4_decode_status, kDevErrPage);
     }
-    none0 = __ballot_sync(0xffffffffu, src0 == nullptr);
-    none1 = __ballot_sync(0xffffffffu, src1 == nullptr);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; j += 2)
+      asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(places + lane * 32 + j * 8), "l"(at[j]), "l"(at[j + 1])
+                   : "memory");
+    __syncwarp();
+    absent = __ballot_sync(0xffffffffu, lost);
+    moving = __ballot_sync(0xffffffffu, change);
   };
-  unsigned gone = 0;  // per ring slot: bit 2s block 0, bit 2s + 1 block 1 is not there
-  auto issue = [&](int k) {  // the warp's tile k
-    const int i = k & 31, slot = k % kDepth;
-    if (i == 0 && k > 0) resolve(k);
-    gone = (gone & ~(3u << (2 * slot))) | ((none0 >> i) & 1u) << (2 * slot) |
-           ((none1 >> i) & 1u) << (2 * slot + 1);
-    if (lane == i) {
-      const uint32_t dst = ring + slot * kTileBytes, mb = smem_u32(&bar[slot]);
-      mbar_arrive_expect_tx(&bar[slot], (src0 ? kBlockBytes : 0) + (src1 ? kBlockBytes : 0));
-      if (src0 && src1 == src0 + kBlockBytes) {
-        bulk_load(dst, src0, kTileBytes, mb);
+  auto issue = [&](int y) {  // tile y, or nothing behind the last; always one group
+    if (y < x1) {
+      const int i = (y - x0) & 31, slot = (y - x0) % kDepth;
+      const uint32_t to = ring + slot * kTileBytes + lane * 16;
+      const uint4 e = lds128(places + i * 32);
+      if (__builtin_expect((absent | gone) != 0, 0)) {
+        const uint4 f = lds128(places + i * 32 + 16);
+        const unsigned b0 = e.x >> 3 & 1u, b1 = e.z >> 3 & 1u, b2 = f.x >> 3 & 1u, b3 = f.z >> 3 & 1u;
+        const unsigned blocks = by_block ? b0 | b1 << 1 | b2 << 2 | b3 << 3 : b0 * 3u | b1 * 12u;
+        gone = (gone & ~(15u << (4 * slot))) | blocks << (4 * slot);
+      }
+      auto copy = [&](uint32_t lo, uint32_t hi, uint32_t dst) {
+        const char* from = reinterpret_cast<const char*>(static_cast<unsigned long long>(hi) << 32 | (lo & ~15u)) + lane * 16;
+        const int size = static_cast<int>(lo & 3u) * kBlockBytes - lane * 16;
+#pragma unroll
+        for (int u = 0; u < 2 * kBlockBytes; u += 512)
+          if (u < size) copy16(dst + u, from + u);
+      };
+      if (by_block) {
+        const uint4 f = lds128(places + i * 32 + 16);
+        copy(e.x, e.y, to);
+        copy(e.z, e.w, to + kBlockBytes);
+        copy(f.x, f.y, to + 2 * kBlockBytes);
+        copy(f.z, f.w, to + 3 * kBlockBytes);
       } else {
-        if (src0) bulk_load(dst, src0, kBlockBytes, mb);
-        if (src1) bulk_load(dst + kBlockBytes, src1, kBlockBytes, mb);
+        copy(e.x, e.y, to);
+        copy(e.z, e.w, to + 2 * kBlockBytes);
       }
     }
+    commit_copies();
   };
-  int issued = 0;
-  resolve(0);
+  int issued = x0;
+  resolve(x0);
   if (early) {  // tiles that no earlier kernel on the stream still writes
-    const unsigned steady = __ballot_sync(0xffffffffu, stable);
-    while (issued < kDepth && issued < mine && (steady >> issued & 1u)) issue(issued++);
+    for (; issued < x0 + kDepth - 1 && !(moving >> (issued - x0) & 1u); ++issued) issue(issued);
     pdl_wait();
   }
-  while (issued < kDepth && issued < mine) issue(issued++);
+  for (; issued < x0 + kDepth - 1; ++issued) issue(issued);
 
-  // ---- the segments: the parts of (sequence, head, row block) in [x0, x1) ----
-  int done = 0;    // tiles of this warp consumed
-  int stuck = -1;  // the tile whose copy did not come
-  bool ok = true;
-  Seq s = load_seq<NT>(p, b);
-  int x = x0;
-  while (x < x1) {
+  // ---- the warp's segments: its parts of the units (sequence, head, row block) in [x0, x1) ----
+  for (int x = x0; x < x1;) {
+    Seq s = load_seq<NT>(p, b);
     while (x >= base + s.total(p.nkv)) {
       base += s.total(p.nkv);
       s = load_seq<NT>(p, ++b);
     }
     const int unit = (x - base) / s.tiles;
-    const int u0 = base + unit * s.tiles, u1 = u0 + s.tiles;  // the unit's tiles
-    const int seg_end = min(u1, x1);
-    const int kvh = unit / s.rb, r0 = (unit - kvh * s.rb) * C::kRows;
-    const int live = min(C::kRows, s.rows - r0);
-
-    // Query fragments: column n = lane / 4 of each n8 tile; k pairs (j, j + 4) of dims 32 grp + 8t.
-    uint32_t qf[NT][4][4];
-    float qs[NT][4][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 8 + g;
-      const int i = r / p.group;
-      const bf16* src = p.q + b * p.q_sb + i * p.q_st + (kvh * p.group + r - i * p.group) * p.q_sh + 8 * t;
-#pragma unroll
-      for (int grp = 0; grp < 4; ++grp) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < s.rows) v = *reinterpret_cast<const uint4*>(src + 32 * grp);
-        qf[nt][grp][0] = __byte_perm(v.x, v.z, 0x5410);
-        qf[nt][grp][1] = __byte_perm(v.x, v.z, 0x7632);
-        qf[nt][grp][2] = __byte_perm(v.y, v.w, 0x5410);
-        qf[nt][grp][3] = __byte_perm(v.y, v.w, 0x7632);
-        float f[8];
-        unpack8(v, f);
-        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qs[nt][grp][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-        qs[nt][grp][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      }
-    }
+    const int u0 = base + unit * s.tiles;  // the unit's first tile
+    const int seg_end = min(u0 + s.tiles, x1);
+    const int kvh = unit / s.rb;
+    const int r0 = (unit - kvh * s.rb) * C::kRows;
+    // Tokens past it are not seen by every row of the segment.
+    const int all_see = static_cast<int>(min(max(s.qpos + r0 / p.group, -1ll), s.kv_end - 1ll));
+    uint32_t qf[NT][4][2], qm[NT][2];
+    float fr[NT];
     Acc<NT> A;
+    // Query fragments: column lane / 4 of an n8 tile is the hi (even) or lo part of row lane / 8, its k
+    // bytes the dims 32 grp + 8t + {0, 2, 4, 6} and + {1, 3, 5, 7}; scores come out times 2^-9 2^e.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) A.l[nt][e] = 0.f, A.m[nt][e] = -INFINITY;
+      const int r = r0 + nt * 4 + (g >> 1);
+      const int i = r / p.group;
+      const bf16* from = p.q + b * p.q_sb + i * p.q_st + (kvh * p.group + r - i * p.group) * p.q_sh + 8 * t;
+      uint4 v[4];
+      uint32_t big = 0;
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp) {
-        A.pm[nt][grp][0] = A.pm[nt][grp][1] = 0.f;
+        v[grp] = r < s.rows ? *reinterpret_cast<const uint4*>(from + 32 * grp) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) A.o[nt][grp][0][i] = A.o[nt][grp][1][i] = 0.f;
+        for (int d = 0; d < 4; ++d) big = __vmaxu2(big, word(v[grp], d) & 0x7fff7fffu);
       }
+      big = max(big >> 16, big & 0xffffu);  // magnitudes of bf16 numbers compare as integers
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // 2^up with the row's maximum times 2^up in [128, 256); for a row of zeros any power will do
+      const int up = min(134 - static_cast<int>(big >> 7), 100);
+      const float f = __uint_as_float(static_cast<uint32_t>(127 + up + (g & 1) * 4) << 23);
+      float qs[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) A.ps[nt][0][i] = A.ps[nt][1][i] = 0.f;
-    }
-    const long long first_lim = s.qpos + r0 / p.group;  // last key of the segment's first row
-    bool any = false;
-    for (; done < mine && x0 + warp + done * kWarps < seg_end; ++done) {
-      const int slot = done % kDepth;
-      const int tok = (x0 + warp + done * kWarps - u0) * kTile;
-      if (ok) ok = mbar_wait(&bar[slot], (done / kDepth) & 1, &g_int4_decode_status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok && stuck < 0) stuck = done;
-      if (ok) {
-        any = true;
-        const uint32_t at = ring + slot * kTileBytes;
-        const unsigned bad = gone >> (2 * slot) & 3u;
-        if (bad || tok + kTile > s.kv_end || tok + kTile - 1 > first_lim) {
-          int lim[NT][2];
+      for (int grp = 0; grp < 4; ++grp) {
+        uint32_t k[2] = {0, 0};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = r0 + nt * 8 + 2 * t + e;
-              const long long last = min(s.qpos + r / p.group, static_cast<long long>(s.kv_end) - 1);
-              lim[nt][e] = r < s.rows ? static_cast<int>(max(last, -1ll)) : -1;
-            }
-          tile_step<NT, true>(at, qf, qs, A, p.scale_log2, lim, tok, !(bad & 1u), !(bad & 2u));
-        } else {
-          const int lim[NT][2] = {};
-          tile_step<NT, false>(at, qf, qs, A, p.scale_log2, lim, tok, true, true);
+        for (int d = 0; d < 4; ++d) {  // dims 2d (low half) and 2d + 1
+          // hi: the upper four significant bits; lo: the other four, both exact in bf16
+          const uint32_t w = word(v[grp], d), hi = w & 0xfff0fff0u;
+          const __nv_bfloat162 lo = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w),
+                                            *reinterpret_cast<const __nv_bfloat162*>(&hi));
+          const uint32_t e = g & 1 ? *reinterpret_cast<const uint32_t*>(&lo) : hi;
+          const uint32_t two = e4m3x2(lo_bf16(e) * f, hi_bf16(e) * f);  // byte 0: dim 2d, byte 1: dim 2d + 1
+          k[0] |= (two & 0xffu) << (8 * d);
+          k[1] |= (two >> 8) << (8 * d);
         }
-        __syncwarp();
-        if (issued < mine) issue(issued++);
+        qf[nt][grp][0] = k[0];
+        qf[nt][grp][1] = k[1];
+        // The sum of the row's dims in the group, as held: a product with ones gives columns 2t, 2t + 1.
+        constexpr uint32_t kOnes = 0x38383838u;
+        const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
+        float c[4];
+        mma_e4m3(c, ones, k[0], k[1], 0.f, 0.f, 0.f, 0.f);
+        qs[grp] = fmaf(c[1], 0.0625f, c[0]) * (1.f / kCodeUnit);
       }
+      // Column g of the product with mids and scales: the row's sums if g is even, else zeros; k bytes as
+      // in tile_step.
+      float z[4];
+#pragma unroll
+      for (int grp = 0; grp < 4; ++grp) z[grp] = __shfl_sync(0xffffffffu, qs[grp], g >> 1);
+      float z0 = t & 1 ? z[2] : z[0], z1 = t & 1 ? z[3] : z[1], y0 = -7.5f * z0, y1 = -7.5f * z1;
+      if (t & 2) {
+        z0 -= __bfloat162float(__float2bfloat16_rn(z0)), z1 -= __bfloat162float(__float2bfloat16_rn(z1));
+        y0 -= __bfloat162float(__float2bfloat16_rn(y0)), y1 -= __bfloat162float(__float2bfloat16_rn(y1));
+      }
+      qm[nt][0] = g & 1 ? 0u : pack_bf16x2(z0, z1);
+      qm[nt][1] = g & 1 ? 0u : pack_bf16x2(y0, y1);
+      fr[nt] = p.scale_log2 * kCodeUnit * __uint_as_float(static_cast<uint32_t>(127 - __shfl_sync(0xffffffffu, up, 8 * t)) << 23);
+      A.l[nt] = 0.f, A.off[nt] = 0.f, A.top[nt] = -INFINITY;
+      A.pm[nt][0] = A.pm[nt][1] = 0;
+    }
+#pragma unroll
+    for (int c = 0; c < Acc<NT>::kCols; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp) A.o[c][grp][0][j] = A.o[c][grp][1][j] = 0.f;
+        A.xs[c][0][j] = A.xs[c][NT > 1][j] = 0.f;
+      }
+    A.sf[0] = A.sf[1] = dup(__uint_as_float(253u << 23));  // the first tile sets it
+    // ---- its tiles ----
+    for (; x < seg_end; ++x) {
+      if (__builtin_expect((issued - x0 & 31) == 0, 0)) resolve(issued);
+      issue(issued++);
+      wait_copies<kDepth - 1>();
+      __syncwarp();
+      const int slot = (x - x0) % kDepth;
+      const int tok = (x - u0) * kTile;
+      const unsigned there = ~gone >> (4 * slot) & 15u;
+      const bool masked = there != 15u || tok + kTile - 1 > all_see;
+      int lim[NT];
+      if (__builtin_expect(masked, 0)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int r = r0 + nt * 4 + t;
+          const long long last = min(s.qpos + r / p.group, static_cast<long long>(s.kv_end) - 1);
+          lim[nt] = r < s.rows ? static_cast<int>(max(last, -1ll)) : -1;
+        }
+      }
+      tile_step<NT>(ring + slot * kTileBytes, qf, qm, A, fr, masked, lim, tok, there);
+      __syncwarp();
     }
 
-    // ---- the warps' parts of the segment meet in shared memory ----
+    const bool from_before = x0 > u0, goes_on = seg_end < u0 + s.tiles;
+    const int which = 2 * warp + (from_before ? 0 : 1);
+    if ((from_before || goes_on) && lane == 0) edge[which] = u0;
+    const int live = min(C::kRows, s.rows - r0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const float2 pm0 = both(A.pm[nt][0]), pm1 = both(A.pm[nt][1]);
+      float l = A.l[nt], pm[4] = {pm0.x, pm0.y, pm1.x, pm1.y};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float l = A.l[nt][e], pm[4];
+      for (int o = 4; o <= 16; o <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-        for (int grp = 0; grp < 4; ++grp) pm[grp] = A.pm[nt][grp][e];
+        for (int grp = 0; grp < 4; ++grp) pm[grp] += __shfl_xor_sync(0xffffffffu, pm[grp], o);
+      }
+      const int row = nt * 4 + t;
+      const bool mine = !from_before && !goes_on;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (!mine && g == 0) ml[which * C::kRows + row] = make_float2(A.off[nt], l);
+      const int i = (r0 + row) / p.group, h = kvh * p.group + r0 + row - i * p.group;
+      bf16* to = p.out + b * p.o_sb + i * p.o_st + h * p.o_sh + 4 * g;
 #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) {
-          l += __shfl_xor_sync(0xffffffffu, l, o);
-#pragma unroll
-          for (int grp = 0; grp < 4; ++grp) pm[grp] += __shfl_xor_sync(0xffffffffu, pm[grp], o);
-        }
-        const int row = nt * 8 + 2 * t + e;
-        if (g == 0) ml[warp * C::kRows + row] = make_float2(A.m[nt][e], l);
-        if (any && row < live) {
-#pragma unroll
-          for (int grp = 0; grp < 4; ++grp) {
-            const float add = pm[grp] - kShift * A.ps[nt][grp >> 1][(grp & 1) * 2 + e];
-            const float4 v = make_float4(A.o[nt][grp][0][e] + add, A.o[nt][grp][0][2 + e] + add,
-                                         A.o[nt][grp][1][e] + add, A.o[nt][grp][1][2 + e] + add);
-            // float4 number 8 grp + g of the row, its place xored with the row pair: no bank conflict
-            const int c4 = (8 * grp + g) ^ (2 * t);
-            *reinterpret_cast<float4*>(red + (warp * C::kRows + row) * kHD + c4 * 4) = v;
-          }
+      for (int grp = 0; grp < 4; ++grp) {
+        const float4 v = chunk_of<NT>(A, nt, grp, pm[grp]);
+        if (!mine) {
+          // float4 number 8 grp + g of the row, its place xored with the row: no bank conflict
+          *reinterpret_cast<float4*>(part_row(which, row) + ((8 * grp + g) ^ (2 * t)) * 4) = v;
+        } else if (row < live) {
+          *reinterpret_cast<uint2*>(to + 32 * grp) =
+              make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
         }
       }
     }
-    if (!ok && lane == 0) *failed = 1;
-    __syncthreads();
-    const bool whole = x <= u0 && seg_end == u1;
-    const int part = 2 * blockIdx.x + (x == x0 ? 0 : 1);
-    if (!*failed)
-      for (int i = tid; i < live * (kHD / 4); i += kThreads) {
-        const int row = i / (kHD / 4), c4 = i % (kHD / 4);
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w * C::kRows + row].x);
-        float L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 v = ml[w * C::kRows + row];
-          if (v.y == 0.f) continue;  // nothing of this warp (a NaN goes on)
-          const float f = ex2(v.x - M);
-          L += f * v.y;
-          const float4 u = *reinterpret_cast<const float4*>(
-              red + (w * C::kRows + row) * kHD + (c4 ^ (row & 6)) * 4);
-          o.x += f * u.x;
-          o.y += f * u.y;
-          o.z += f * u.z;
-          o.w += f * u.w;
-        }
-        if (whole) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          write_row4(p, b, kvh, r0 + row, c4 * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-        } else {
-          *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(part) * C::kRows + row) * kHD + c4 * 4) = o;
-          if (c4 == 0) p.part_ml[part * C::kRows + row] = make_float2(M, L);
-        }
-      }
-    x = seg_end;
-    if (x < x1) __syncthreads();  // the next segment overwrites red and ml
   }
-  // After a failed wait the copies still in flight must land before the shared memory goes.
-  if (!ok)
-    for (; stuck < issued; ++stuck) mbar_wait(&bar[stuck % kDepth], (stuck / kDepth) & 1, nullptr);
+  __syncthreads();
+
+  // ---- units that the CTA's warps share, added up row by row by warps in turn ----
+  const int e = lane < 2 * kWarps ? edge[lane] : -1;
+  const int cta0 = range[0].x0, cta1 = range[kWarps].x0;
+  if (p.direct && cta0 == cta1) {  // rows that see no key
+    const Seq z = load_seq<NT>(p, blockIdx.y);
+    if (static_cast<int>(blockIdx.x) >= z.units(p.nkv)) return;
+    const int head = blockIdx.x / z.rb, row0 = (blockIdx.x - head * z.rb) * C::kRows;
+    for (int row = warp; row < min(C::kRows, z.rows - row0); row += kWarps)
+      write_row4(p, blockIdx.y, head, row0 + row, lane * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  unsigned todo = __ballot_sync(0xffffffffu, e >= 0);
+  for (int turn = 0; todo; ) {
+    const int first = __ffs(todo) - 1, unit0 = __shfl_sync(0xffffffffu, e, first);
+    const unsigned parts = __ballot_sync(0xffffffffu, e == unit0);
+    todo &= ~parts;
+    int ub = range[first >> 1].seq, ubase = range[first >> 1].base;  // its sequence, or one before it
+    Seq us = load_seq<NT>(p, ub);
+    while (unit0 >= ubase + us.total(p.nkv)) {
+      ubase += us.total(p.nkv);
+      us = load_seq<NT>(p, ++ub);
+    }
+    const int unit = (unit0 - ubase) / us.tiles, head = unit / us.rb, row0 = (unit - head * us.rb) * C::kRows;
+    const int live = min(C::kRows, us.rows - row0);
+    const bool whole = cta0 <= unit0 && unit0 + us.tiles <= cta1;
+    const int part = 2 * blockIdx.x + (cta0 >= unit0 ? 0 : 1);
+    for (int row = 0; row < live; ++row, ++turn) {
+      if (turn % kWarps != warp) continue;
+      float2 v = make_float2(-INFINITY, 0.f);
+      if (parts >> lane & 1u) v = ml[lane * C::kRows + row];
+      float M = v.y == 0.f ? -INFINITY : v.x;  // a part that sees no key of the row does not count
+#pragma unroll
+      for (int o = 1; o <= 8; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float f = v.y == 0.f ? 0.f : ex2(v.x - M);
+      float L = f * v.y;
+#pragma unroll
+      for (int o = 1; o <= 8; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      M = __shfl_sync(0xffffffffu, M, 0);
+      L = __shfl_sync(0xffffffffu, L, 0);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (unsigned left = parts; left; left &= left - 1) {
+        const int w = __ffs(left) - 1;
+        const float fw = __shfl_sync(0xffffffffu, f, w);
+        const float4 u = *reinterpret_cast<const float4*>(part_row(w, row) + (lane ^ (2 * (row & 3))) * 4);
+        o = make_float4(o.x + fw * u.x, o.y + fw * u.y, o.z + fw * u.z, o.w + fw * u.w);
+      }
+      if (whole) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        write_row4(p, ub, head, row0 + row, lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(part) * C::kRows + row) * kHD + lane * 4) = o;
+        if (lane == 0) p.part_ml[part * C::kRows + row] = make_float2(M, L);
+      }
+    }
+  }
 }
 
 // The rows whose tiles were divided between CTAs: one CTA per output row, whose warps take the parts
@@ -612,8 +876,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int R = blockIdx.x;
   const int h = R % p.nh, i = (R / p.nh) % p.q_len, b = R / (p.nh * p.q_len);
-  int base = 0;
-  const int total = list_total<NT>(p, b, &base);
+  Prefix f;
+  int cost0 = 0;  // of the sequences before b
+  for (int c = 0; c < p.batch; c += 32) {
+    load_prefix<NT>(p, f, c);
+    if (b >= c && b < c + 32) cost0 = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl - f.cost, b - c);
+  }
+  const int cost = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl, 31);
   const Seq s = load_seq<NT>(p, b);
   if (p.stable_prefix) pdl_wait();
   const int kvh = h / p.group, r = i * p.group + h - kvh * p.group;
@@ -622,14 +891,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
     if (warp == 0) write_row4(p, b, kvh, r, lane * 4, make_float4(0.f, 0.f, 0.f, 0.f));
     return;
   }
-  const int n = active_ctas(total, p.ctas);
-  const int u0 = base + (kvh * s.rb + r / C::kRows) * s.tiles;
-  const int c0 = cta_of(total, n, u0), c1 = cta_of(total, n, u0 + s.tiles - 1);
+  const Division d(cost, p.ctas);
+  const int u0 = cost0 + (kvh * s.rb + r / C::kRows) * (s.tiles + kUnitCost);  // the unit's first position
+  const int c0 = d.worker(u0 + kUnitCost) / kWarps, c1 = d.worker(u0 + kUnitCost + s.tiles - 1) / kWarps;
   if (c0 == c1) return;  // written whole
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
-    const int part = 2 * c + (first_tile(total, n, c) >= u0 ? 0 : 1);
+    const int part = 2 * c + (d.first(c * kWarps) >= u0 ? 0 : 1);
     const int64_t row = static_cast<int64_t>(part) * C::kRows + r % C::kRows;
     const float2 v = p.part_ml[row];
     const float4 u = *reinterpret_cast<const float4*>(p.part_o + row * kHD + lane * 4);
@@ -673,11 +942,11 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
     return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->num_qo_heads % a->num_kv_heads != 0) return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->batch > 65535) return SOLORT_ERR_UNSUPPORTED;
-  // One n8 tile of rows where the rows fit it (two CTAs per SM), else blocks of 16 rows.
+  // One n8 tile, four rows, where they fit it (two CTAs per SM), else blocks of eight rows.
   const int64_t rows = static_cast<int64_t>(a->q_len) * (a->num_qo_heads / a->num_kv_heads);
-  pl->nt = rows <= 8 ? 1 : 2;
-  const int64_t rb = (rows + 8 * pl->nt - 1) / (8 * pl->nt);
-  const int64_t tiles = (static_cast<int64_t>(a->max_kv_len) + kTile - 1) / kTile;
+  pl->nt = rows <= 4 ? 1 : 2;
+  const int64_t rb = (rows + 4 * pl->nt - 1) / (4 * pl->nt);
+  const int64_t tiles = (static_cast<int64_t>(a->max_kv_len) + kTile - 1) / kTile + kUnitCost;
   const int64_t units = rb * a->num_kv_heads;
   const int64_t out_rows = static_cast<int64_t>(a->batch) * a->q_len * a->num_qo_heads;
   const int64_t limit = (1ll << 31) - 1;
@@ -688,15 +957,15 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   int rc = current_device_info(&di);
   if (rc != SOLORT_OK) return rc;
   pl->rb = static_cast<int>(rb);
-  pl->direct = tiles <= kDirectTiles && a->num_ctas == 0;
+  pl->direct = tiles - kUnitCost <= kDirectTiles && a->num_ctas == 0;
   if (pl->direct) return SOLORT_OK;
-  const int64_t most = (tiles * units * a->batch + kMinTiles - 1) / kMinTiles;
+  const int64_t most = (tiles * units * a->batch + kWarps - 1) / kWarps;
   const int64_t wave = a->num_ctas > 0 ? a->num_ctas
                                        : static_cast<int64_t>(di.sm_count) *
                                              (pl->nt == 1 ? Cfg<1>::kCtasPerSm : Cfg<2>::kCtasPerSm);
   if (wave > (1 << 20)) return SOLORT_ERR_UNSUPPORTED;
   pl->ctas = static_cast<int>(most < wave ? most : wave);
-  const size_t parts = static_cast<size_t>(2) * pl->ctas * 8 * pl->nt;
+  const size_t parts = static_cast<size_t>(2) * pl->ctas * 4 * pl->nt;
   pl->o_bytes = parts * kHD * 4;
   pl->ws_bytes = align_up(pl->o_bytes + parts * 8, 256);
   return SOLORT_OK;
