@@ -47,11 +47,8 @@ namespace i4 {
 
 constexpr int kTile = 32;                     // tokens of a tile: four blocks
 constexpr int kTileBytes = 4 * kBlockBytes;   // 5120
-constexpr int kDepth = 3;                     // tiles of a warp in shared memory
-constexpr int kWarps = 6;
-constexpr int kThreads = kWarps * 32;
 constexpr int kUnitCost = 2;                  // tiles' worth of set-up of a (sequence, head, row block)
-constexpr int kDirectTiles = 2 * kWarps;      // up to this many tiles a (sequence, head) is one CTA
+constexpr int kDirectTiles = 16;              // up to this many tiles a (sequence, head) is one CTA
 // A row's running maximum is raised only when a score passes it by 2^kLazy; p is 2^kPShift there, so
 // that x stays below 2^15, inside f16.
 constexpr float kLazy = 7.f;
@@ -59,8 +56,14 @@ constexpr float kPShift = 15.f - kLazy;
 constexpr float kCodeUnit = 512.f;         // a key code's e4m3 value is c / 512
 constexpr float kValueUnit = 16777216.f;   // a value code's f16 value is c 2^-24, or 16 c 2^-24
 
-template <int NT>  // n8 tiles: four query rows each
+// NT n8 tiles of four query rows each. One: 160 registers a thread and 111 KB, so that two CTAs of six
+// warps share an SM. Two: one CTA of eight warps with all the registers that they can have.
+template <int NT>
 struct Cfg {
+  static constexpr int kWarps = 6;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kCtasPerSm = 2;
+  static constexpr int kDepth = NT == 1 ? 3 : 2;  // tiles of a warp in shared memory
   static constexpr int kRows = 4 * NT;
   static constexpr int kRing = kWarps * kDepth * kTileBytes;
   static constexpr int kRed = kWarps * kRows * kHD * 4;
@@ -71,7 +74,6 @@ struct Cfg {
   static constexpr int kOffRange = kOffEdge + 2 * kWarps * 4;
   static constexpr int kOffPlaces = (kOffRange + (kWarps + 1) * 12 + 15) / 16 * 16;  // [warp][32 tiles][4]
   static constexpr int kSmem = kOffPlaces + kWarps * 32 * 32;
-  static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
 };
 static_assert(Cfg<1>::kSmem <= 115712, "two CTAs per SM");
 
@@ -88,7 +90,9 @@ struct Params {
   const int64_t* q_pos;
   const int32_t* q_lens;
   float* part_o;    // [2 * ctas][rows][128], not normalised
-  float2* part_ml;  // [2 * ctas][rows] running max (log2 domain) and sum
+  float2* part_ml;  // [2 * ctas][rows] reference (log2 domain) and sum
+  int2* span;       // [batch][nkv][row block] its first part, and the CTA of its last
+  int rb;           // row blocks of q_len tokens
   int batch, q_len, nh, nkv, group, max_kv_len;
   int direct;  // grid (head and row block, sequence): no parts
   int ctas;
@@ -150,16 +154,12 @@ __device__ __forceinline__ void load_prefix(const Params& p, Prefix& f, int firs
 // one position more than the others.
 struct Division {
   int n, each, more;
-  __device__ __forceinline__ Division(int cost, int ctas) {
-    n = max(1, min(ctas, (cost + kWarps - 1) / kWarps)) * kWarps;
+  __device__ __forceinline__ Division(int cost, int ctas, int warps) {
+    n = max(1, min(ctas, (cost + warps - 1) / warps)) * warps;
     each = cost / n;
     more = cost - each * n;
   }
   __device__ __forceinline__ int first(int w) const { return w * each + min(w, more); }
-  __device__ __forceinline__ int worker(int x) const {
-    const int split = more * (each + 1);
-    return x < split ? x / (each + 1) : more + (x - split) / each;
-  }
 };
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -513,8 +513,9 @@ struct Range {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
   using C = Cfg<NT>;
+  constexpr int kWarps = C::kWarps, kDepth = C::kDepth;
   extern __shared__ __align__(128) uint8_t smem[];
   // What a warp leaves of a unit that it shares with other warps: its first unit's (begun before the
   // warp's range) in `red`, and its last's (begun in it, going on behind it) where its ring was.
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(c
       Prefix f;
       for (int c = 0; c < p.batch; c += 32) load_prefix<NT>(p, f, c);
       const int cost = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl, 31);
-      const Division d(cost, p.ctas);
+      const Division d(cost, p.ctas, kWarps);
       const int X = d.first(min(static_cast<int>(blockIdx.x) * kWarps + min(lane, kWarps), d.n));
       r.x0 = f.tiles_run + __shfl_sync(0xffffffffu, f.tiles_incl, 31);  // the end of the list
       r.seq = p.batch;
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(c
       float qs[4];
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp) {
-        uint32_t k[2] = {0, 0};
+        uint32_t two[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) {  // dims 2d (low half) and 2d + 1
           // hi: the upper four significant bits; lo: the other four, both exact in bf16
@@ -710,10 +711,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(c
           const __nv_bfloat162 lo = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w),
                                             *reinterpret_cast<const __nv_bfloat162*>(&hi));
           const uint32_t e = g & 1 ? *reinterpret_cast<const uint32_t*>(&lo) : hi;
-          const uint32_t two = e4m3x2(lo_bf16(e) * f, hi_bf16(e) * f);  // byte 0: dim 2d, byte 1: dim 2d + 1
-          k[0] |= (two & 0xffu) << (8 * d);
-          k[1] |= (two >> 8) << (8 * d);
+          two[d] = e4m3x2(lo_bf16(e) * f, hi_bf16(e) * f);
         }
+        const uint32_t w0 = __byte_perm(two[0], two[1], 0x5410), w1 = __byte_perm(two[2], two[3], 0x5410);
+        const uint32_t k[2] = {__byte_perm(w0, w1, 0x6420), __byte_perm(w0, w1, 0x7531)};
         qf[nt][grp][0] = k[0];
         qf[nt][grp][1] = k[1];
         // The sum of the row's dims in the group, as held: a product with ones gives columns 2t, 2t + 1.
@@ -772,6 +773,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(c
     }
 
     const bool from_before = x0 > u0, goes_on = seg_end < u0 + s.tiles;
+    if (!p.direct && lane == 0) {
+      int2* span = p.span + (b * p.nkv + kvh) * p.rb + (unit - kvh * s.rb);
+      if (!from_before) span->x = 2 * blockIdx.x + (range[0].x0 >= u0 ? 0 : 1);
+      if (!goes_on) span->y = blockIdx.x;
+    }
     const int which = 2 * warp + (from_before ? 0 : 1);
     if ((from_before || goes_on) && lane == 0) edge[which] = u0;
     const int live = min(C::kRows, s.rows - r0);
@@ -864,8 +870,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(c
 }
 
 // The rows whose tiles were divided between CTAs: one CTA per output row, whose warps take the parts
-// in turn. Rows that see no key are zeroed here too. Bound by its latency.
-constexpr int kMergeWarps = 4;
+// in turn. Rows that see no key are zeroed here too. Bound by its latency: two round trips to L2, and
+// what the many rows of a large batch, mostly written whole already, take to leave.
+constexpr int kMergeWarps = 8;
+constexpr int kMergeLoads = 5;  // parts of a warp whose loads are in flight together: 40 parts a round trip
 template <int NT>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p) {
   using C = Cfg<NT>;
@@ -874,50 +882,59 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
   pdl_launch_dependents();
   if (!p.stable_prefix) pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
   const int R = blockIdx.x;
   const int h = R % p.nh, i = (R / p.nh) % p.q_len, b = R / (p.nh * p.q_len);
-  Prefix f;
-  int cost0 = 0;  // of the sequences before b
-  for (int c = 0; c < p.batch; c += 32) {
-    load_prefix<NT>(p, f, c);
-    if (b >= c && b < c + 32) cost0 = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl - f.cost, b - c);
-  }
-  const int cost = f.cost_run + __shfl_sync(0xffffffffu, f.cost_incl, 31);
+  const int kvh = h / p.group, r = i * p.group + h - kvh * p.group;
   const Seq s = load_seq<NT>(p, b);
   if (p.stable_prefix) pdl_wait();
-  const int kvh = h / p.group, r = i * p.group + h - kvh * p.group;
+  const int2 span = p.span[(b * p.nkv + kvh) * p.rb + r / C::kRows];
   if (r >= s.rows) return;
   if (s.tiles == 0) {
     if (warp == 0) write_row4(p, b, kvh, r, lane * 4, make_float4(0.f, 0.f, 0.f, 0.f));
     return;
   }
-  const Division d(cost, p.ctas);
-  const int u0 = cost0 + (kvh * s.rb + r / C::kRows) * (s.tiles + kUnitCost);  // the unit's first position
-  const int c0 = d.worker(u0 + kUnitCost) / kWarps, c1 = d.worker(u0 + kUnitCost + s.tiles - 1) / kWarps;
+  const int c0 = span.x >> 1, c1 = span.y;
   if (c0 == c1) return;  // written whole
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
-    const int part = 2 * c + (d.first(c * kWarps) >= u0 ? 0 : 1);
-    const int64_t row = static_cast<int64_t>(part) * C::kRows + r % C::kRows;
-    const float2 v = p.part_ml[row];
-    const float4 u = *reinterpret_cast<const float4*>(p.part_o + row * kHD + lane * 4);
-    if (v.y == 0.f) continue;  // the part sees no key of the row (a NaN goes on)
-    const float m = fmaxf(M, v.x), f0 = L == 0.f ? 0.f : ex2(M - m), f1 = ex2(v.x - m);
+  for (int c = c0 + warp; c <= c1; c += warps * kMergeLoads) {
+    float2 v[kMergeLoads];
+    float4 u[kMergeLoads];
+#pragma unroll
+    for (int j = 0; j < kMergeLoads; ++j) {
+      const int cj = c + j * warps;
+      v[j] = make_float2(-INFINITY, 0.f);
+      u[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (cj <= c1) {
+        const int part = cj == c0 ? span.x : 2 * cj;  // behind its first CTA a unit is the CTA's first
+        const int64_t row = static_cast<int64_t>(part) * C::kRows + r % C::kRows;
+        v[j] = p.part_ml[row];
+        u[j] = *reinterpret_cast<const float4*>(p.part_o + row * kHD + lane * 4);
+      }
+    }
+    float m = M;  // a part that sees no key of the row (sum 0) does not count; a NaN goes on
+#pragma unroll
+    for (int j = 0; j < kMergeLoads; ++j) m = v[j].y == 0.f ? m : fmaxf(m, v[j].x);
+    const float f0 = L == 0.f ? 0.f : ex2(M - m);
     M = m;
-    L = L * f0 + v.y * f1;
-    o = make_float4(o.x * f0 + u.x * f1, o.y * f0 + u.y * f1, o.z * f0 + u.z * f1, o.w * f0 + u.w * f1);
+    L *= f0;
+    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+    for (int j = 0; j < kMergeLoads; ++j) {
+      const float f = v[j].y == 0.f ? 0.f : ex2(v[j].x - m);
+      L += f * v[j].y;
+      o = make_float4(o.x + f * u[j].x, o.y + f * u[j].y, o.z + f * u[j].z, o.w + f * u[j].w);
+    }
   }
   so[warp][lane] = o;
   if (lane == 0) sm[warp] = make_float2(M, L);
   __syncthreads();
   if (warp) return;
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) M = fmaxf(M, sm[w].x);
+  for (int w = 0; w < warps; ++w) M = sm[w].y == 0.f ? M : fmaxf(M, sm[w].x);
   L = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) {
+  for (int w = 0; w < warps; ++w) {
     if (sm[w].y == 0.f) continue;
     const float f = ex2(sm[w].x - M);
     const float4 u = so[w][lane];
@@ -931,7 +948,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
 struct Plan {
   int nt = 1, ctas = 1, rb = 1;
   bool direct = false;
-  size_t o_bytes = 0, ws_bytes = 0;
+  size_t o_bytes = 0, ml_bytes = 0, ws_bytes = 0;
 };
 
 int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
@@ -945,6 +962,7 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   // One n8 tile, four rows, where they fit it (two CTAs per SM), else blocks of eight rows.
   const int64_t rows = static_cast<int64_t>(a->q_len) * (a->num_qo_heads / a->num_kv_heads);
   pl->nt = rows <= 4 ? 1 : 2;
+  const int warps = pl->nt == 1 ? Cfg<1>::kWarps : Cfg<2>::kWarps;
   const int64_t rb = (rows + 4 * pl->nt - 1) / (4 * pl->nt);
   const int64_t tiles = (static_cast<int64_t>(a->max_kv_len) + kTile - 1) / kTile + kUnitCost;
   const int64_t units = rb * a->num_kv_heads;
@@ -959,7 +977,7 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   pl->rb = static_cast<int>(rb);
   pl->direct = tiles - kUnitCost <= kDirectTiles && a->num_ctas == 0;
   if (pl->direct) return SOLORT_OK;
-  const int64_t most = (tiles * units * a->batch + kWarps - 1) / kWarps;
+  const int64_t most = (tiles * units * a->batch + warps - 1) / warps;
   const int64_t wave = a->num_ctas > 0 ? a->num_ctas
                                        : static_cast<int64_t>(di.sm_count) *
                                              (pl->nt == 1 ? Cfg<1>::kCtasPerSm : Cfg<2>::kCtasPerSm);
@@ -967,7 +985,8 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   pl->ctas = static_cast<int>(most < wave ? most : wave);
   const size_t parts = static_cast<size_t>(2) * pl->ctas * 4 * pl->nt;
   pl->o_bytes = parts * kHD * 4;
-  pl->ws_bytes = align_up(pl->o_bytes + parts * 8, 256);
+  pl->ml_bytes = parts * 8;
+  pl->ws_bytes = align_up(pl->o_bytes + pl->ml_bytes + static_cast<size_t>(units) * a->batch * 8, 256);
   return SOLORT_OK;
 }
 
@@ -1001,11 +1020,13 @@ int launch(const Params& prm, const Plan& pl, void* stream) {
   }
   cudaLaunchAttribute attr[1];
   const dim3 grid = pl.direct ? dim3(prm.nkv * pl.rb, prm.batch) : dim3(pl.ctas);
-  cudaLaunchConfig_t cfg = pdl_config(grid, kThreads, C::kSmem, stream, attr);
+  cudaLaunchConfig_t cfg = pdl_config(grid, C::kThreads, C::kSmem, stream, attr);
   if (cudaLaunchKernelEx(&cfg, decode_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   int rc = launch_status();
   if (rc != SOLORT_OK || pl.direct) return rc;
-  cfg = pdl_config(dim3(prm.batch * prm.q_len * prm.nh), kMergeWarps * 32, 0, stream, attr);
+  // Few rows have many parts each, and want many warps; of many rows most have one, and want to leave.
+  const int rows = prm.batch * prm.q_len * prm.nh;
+  cfg = pdl_config(dim3(rows), (rows <= pl.ctas ? kMergeWarps : 2) * 32, 0, stream, attr);
   if (cudaLaunchKernelEx(&cfg, merge_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   return launch_status();
 }
@@ -1077,6 +1098,7 @@ extern "C" int solort_attn_decode_int4(const SolortInt4DecodeArgs* a, void* stre
   if (!pl.direct) {
     p.part_o = static_cast<float*>(a->workspace);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(a->workspace) + pl.o_bytes);
+    p.span = reinterpret_cast<int2*>(static_cast<uint8_t*>(a->workspace) + pl.o_bytes + pl.ml_bytes);
   }
   p.batch = a->batch;
   p.q_len = a->q_len;
@@ -1086,6 +1108,7 @@ extern "C" int solort_attn_decode_int4(const SolortInt4DecodeArgs* a, void* stre
   p.max_kv_len = a->max_kv_len;
   p.direct = pl.direct ? 1 : 0;
   p.ctas = pl.ctas;
+  p.rb = pl.rb;
   p.stable_prefix = (a->flags & SOLORT_DECODE_STABLE_PREFIX) ? 1 : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   return pl.nt == 1 ? i4::launch<1>(p, pl, stream) : i4::launch<2>(p, pl, stream);
