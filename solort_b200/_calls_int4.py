@@ -14,7 +14,7 @@ from solort_b200 import _lib
 from solort_b200._calls import HEAD_DIM, _stream_at
 
 TOKEN_BYTES = 160  # K and V of one token of one KV head: codes, and a scale and a mid per 32 values
-_byref, _vp = ctypes.byref, ctypes.c_void_p
+_byref = ctypes.byref
 _BF16, _I64, _I32, _U8 = torch.bfloat16, torch.int64, torch.int32, torch.uint8
 
 
@@ -55,58 +55,90 @@ def _rows(name: str, t: torch.Tensor, n: int, heads: int) -> None:
 
 
 def _launch(name: str, args, index: int) -> None:
-    fn = getattr(_lib.load(), name)
-    if index == torch.cuda.current_device():
-        rc = fn(_byref(args), _vp(_stream_at(index)))
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.load(), name)
+    if index == _current_device():
+        rc = fn(_byref(args), _stream_at(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(_byref(args), _vp(_stream_at(index)))
+            rc = fn(_byref(args), _stream_at(index))
     if rc:
         _lib.check(rc, name)
 
+
+_FN: dict[str, object] = {}
+# torch's raw getter: what torch.cuda.current_device() returns, less its look at the lazy start (the
+# tensors of a call are on the device already).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+# The conditions of a call are looked at together first, since a decode step's calls are as short as
+# their checks; only where one fails are they gone through one by one, for the error's words.
 
 def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positions, slots, kv_pages,
                 q_out) -> None:
     """The batch attention prologue into the 4-bit cache: the body of
     ``solort_attn::qk_norm_rope_append_int4``. Head counts follow from ``q_out`` and ``kv_pages``."""
-    P = page_size(kv_pages)
-    num_pages, nkv, _ = kv_pages.shape
-    index = _same_device(qkv, ("kv_pages", kv_pages), ("q_out", q_out), ("cos", cos), ("sin", sin),
-                         ("positions", positions), ("slots", slots),
-                         ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight))
-    _need(q_out.dim() == 3, "q_out must be [tokens, num_qo_heads, 128]")
-    t, nh = qkv.shape[0], q_out.shape[1]
-    _rows("q_out", q_out, t, nh)
-    _need(qkv.dtype is _BF16 and qkv.dim() == 2 and qkv.stride(1) == 1 and
-          qkv.shape[1] == (nh + 2 * nkv) * HEAD_DIM,
-          f"qkv must be bf16 [tokens, ({nh} + 2 * {nkv}) * 128] with contiguous rows")
-    for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
-        _need(w.dtype is _BF16 and w.shape == (HEAD_DIM,) and w.stride(0) == 1,
-              f"{name} must be a contiguous bf16 [128] vector")
-    _need(cos.dtype is _BF16 and sin.dtype is _BF16 and cos.dim() == 2 and cos.shape == sin.shape and
-          cos.shape[1] == HEAD_DIM and cos.stride() == sin.stride() and cos.stride(1) == 1,
-          "cos and sin must be bf16 [rows, 128] tables with equal strides and contiguous rows")
-    _vector("positions", positions, _I64, t)
-    _vector("slots", slots, _I64, t)
+    t = qkv.shape[0]
+    pages, cs, outs = kv_pages.shape, cos.shape, q_out.shape
+    index = qkv.get_device()
+    sp, so, sc = kv_pages.stride(), q_out.stride(), cos.stride()
+    P = pages[-1] // TOKEN_BYTES
+    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+            P * TOKEN_BYTES == pages[2] and len(outs) == 3 and len(cs) == 2 and index >= 0 and
+            index == kv_pages.get_device() == q_out.get_device() == cos.get_device() ==
+            sin.get_device() == positions.get_device() == slots.get_device() ==
+            q_norm_weight.get_device() == k_norm_weight.get_device() and
+            _BF16 is qkv.dtype is q_out.dtype is cos.dtype is sin.dtype is q_norm_weight.dtype is
+            k_norm_weight.dtype and _I64 is positions.dtype is slots.dtype and
+            outs == (t, outs[1], HEAD_DIM) and so[2] == 1 and
+            qkv.shape == (t, (outs[1] + 2 * pages[1]) * HEAD_DIM) and qkv.stride(1) == 1 and
+            q_norm_weight.shape == k_norm_weight.shape == (HEAD_DIM,) and
+            q_norm_weight.stride(0) == 1 == k_norm_weight.stride(0) and
+            cs == sin.shape and cs[1] == HEAD_DIM and sc == sin.stride() and sc[1] == 1 and
+            positions.shape == slots.shape == (t,) and
+            (t < 2 or positions.stride(0) == 1 == slots.stride(0))):
+        page_size(kv_pages)
+        _same_device(qkv, ("kv_pages", kv_pages), ("q_out", q_out), ("cos", cos), ("sin", sin),
+                     ("positions", positions), ("slots", slots),
+                     ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight))
+        _need(q_out.dim() == 3, "q_out must be [tokens, num_qo_heads, 128]")
+        _rows("q_out", q_out, t, outs[1])
+        _need(qkv.dtype is _BF16 and qkv.dim() == 2 and qkv.stride(1) == 1 and
+              qkv.shape[1] == (outs[1] + 2 * pages[1]) * HEAD_DIM,
+              f"qkv must be bf16 [tokens, ({outs[1]} + 2 * {pages[1]}) * 128] with contiguous rows")
+        for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
+            _need(w.dtype is _BF16 and w.shape == (HEAD_DIM,) and w.stride(0) == 1,
+                  f"{name} must be a contiguous bf16 [128] vector")
+        _vector("positions", positions, _I64, t)
+        _vector("slots", slots, _I64, t)
+        raise RuntimeError("cos and sin must be bf16 [rows, 128] tables with equal strides and "
+                           "contiguous rows")
     _launch("solort_attn_qk_norm_rope_append_int4", _lib.SolortInt4AppendArgs(
-        qkv.data_ptr(), qkv.stride(0), t, nh, nkv, HEAD_DIM, q_norm_weight.data_ptr(),
-        k_norm_weight.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0],
-        positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-        kv_pages.data_ptr(), kv_pages.stride(0), kv_pages.stride(1), P, num_pages), index)
+        qkv.data_ptr(), qkv.stride(0), t, outs[1], pages[1], HEAD_DIM, q_norm_weight.data_ptr(),
+        k_norm_weight.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), sc[0], cs[0],
+        positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), so[0], so[1],
+        kv_pages.data_ptr(), sp[0], sp[1], P, pages[0]), index)
 
 
 def _key_value(what, key, value, slots, kv_pages):
-    P = page_size(kv_pages)
-    num_pages, nkv, _ = kv_pages.shape
-    index = _same_device(kv_pages, ("key", key), ("value", value), ("slots", slots))
-    n = slots.shape[0] if slots.dim() == 1 else -1
-    _vector("slots", slots, _I64, n)
-    _rows("key", key, n, nkv)
-    _rows("value", value, n, nkv)
-    return index, what(
-        key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0),
-        value.stride(1), n, nkv, HEAD_DIM, slots.data_ptr(), kv_pages.data_ptr(), kv_pages.stride(0),
-        kv_pages.stride(1), P, num_pages)
+    pages, sp = kv_pages.shape, kv_pages.stride()
+    sk, sv, index, n = key.stride(), value.stride(), key.get_device(), slots.numel()
+    P = pages[-1] // TOKEN_BYTES
+    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+            P * TOKEN_BYTES == pages[2] and index >= 0 and
+            index == value.get_device() == slots.get_device() == kv_pages.get_device() and
+            _BF16 is key.dtype is value.dtype and slots.dtype is _I64 and slots.shape == (n,) and
+            (n < 2 or slots.stride(0) == 1) and
+            key.shape == value.shape == (n, pages[1], HEAD_DIM) and sk[2] == 1 == sv[2]):
+        page_size(kv_pages)
+        _same_device(kv_pages, ("key", key), ("value", value), ("slots", slots))
+        _vector("slots", slots, _I64, n)
+        _rows("key", key, n, pages[1])
+        _rows("value", value, n, pages[1])
+    return index, what(key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], n, pages[1],
+                       HEAD_DIM, slots.data_ptr(), kv_pages.data_ptr(), sp[0], sp[1], P, pages[0])
 
 
 def store_into(key, value, slots, kv_pages) -> None:
@@ -124,44 +156,57 @@ def load_into(kv_pages, slots, key, value) -> None:
 def decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: float | None, q_lens,
                 num_ctas: int, stable_prefix: bool):
     """Checked and packed arguments of a decode call without its workspace, and the device index."""
-    P = page_size(kv_pages)
-    num_pages, nkv, _ = kv_pages.shape
-    index = _same_device(q, ("kv_pages", kv_pages), ("block_table", block_table), ("q_pos", q_pos),
-                         ("out", out))
-    _need(q.dtype is _BF16 and q.dim() == 4 and q.shape[3] == HEAD_DIM and q.stride(3) == 1,
-          "q must be bf16 [batch, q_len, num_qo_heads, 128] with a contiguous head dim")
-    B, T, H, D = q.shape
-    _need(out.dtype is _BF16 and out.shape == q.shape and out.stride(3) == 1,
-          "out must be bf16, of the shape of q, with a contiguous head dim")
-    _need(block_table.dtype is _I32 and block_table.dim() == 2 and block_table.shape[0] == B and
-          (block_table.shape[1] < 2 or block_table.stride(1) == 1),
-          "block_table must be int32 [batch, max_pages] with contiguous rows")
-    _need(0 < max_kv_len <= block_table.shape[1] * P,
-          f"max_kv_len must be in 1..{block_table.shape[1] * P}, the keys a block-table row can hold, "
-          f"got {max_kv_len}")
-    _vector("q_pos", q_pos, _I64, B)
+    shape, pages, table = q.shape, kv_pages.shape, block_table.shape
+    sq, so, sp, index = q.stride(), out.stride(), kv_pages.stride(), q.get_device()
+    P = pages[-1] // TOKEN_BYTES
+    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+            P * TOKEN_BYTES == pages[2] and len(shape) == 4 and len(table) == 2 and index >= 0 and
+            index == kv_pages.get_device() == block_table.get_device() == q_pos.get_device() ==
+            out.get_device() and _BF16 is q.dtype is out.dtype and block_table.dtype is _I32 and
+            q_pos.dtype is _I64 and shape[3] == HEAD_DIM and sq[3] == 1 and out.shape == shape and
+            so[3] == 1 and table[0] == shape[0] and (table[1] < 2 or block_table.stride(1) == 1) and
+            0 < max_kv_len <= table[1] * P and q_pos.shape == shape[:1] and
+            (shape[0] < 2 or q_pos.stride(0) == 1)):
+        page_size(kv_pages)
+        _same_device(q, ("kv_pages", kv_pages), ("block_table", block_table), ("q_pos", q_pos),
+                     ("out", out))
+        _need(q.dtype is _BF16 and q.dim() == 4 and shape[3] == HEAD_DIM and sq[3] == 1,
+              "q must be bf16 [batch, q_len, num_qo_heads, 128] with a contiguous head dim")
+        _need(out.dtype is _BF16 and out.shape == shape and so[3] == 1,
+              "out must be bf16, of the shape of q, with a contiguous head dim")
+        _need(block_table.dtype is _I32 and len(table) == 2 and table[0] == shape[0] and
+              (table[1] < 2 or block_table.stride(1) == 1),
+              "block_table must be int32 [batch, max_pages] with contiguous rows")
+        _need(0 < max_kv_len <= table[1] * P,
+              f"max_kv_len must be in 1..{table[1] * P}, the keys a block-table row can hold, "
+              f"got {max_kv_len}")
+        _vector("q_pos", q_pos, _I64, shape[0])
     if q_lens is not None:
         _need(q_lens.device == q.device, f"q_lens is on {q_lens.device}, not on {q.device}")
-        _vector("q_lens", q_lens, _I32, B)
-    sq, so = q.stride(), out.stride()
+        _vector("q_lens", q_lens, _I32, shape[0])
     return index, _lib.SolortInt4DecodeArgs(
         q.data_ptr(), sq[0], sq[1], sq[2], out.data_ptr(), so[0], so[1], so[2], kv_pages.data_ptr(),
-        kv_pages.stride(0), kv_pages.stride(1), P, num_pages, block_table.data_ptr(),
-        block_table.stride(0), q_pos.data_ptr(), None if q_lens is None else q_lens.data_ptr(), B, T, H,
-        nkv, D, max_kv_len, D ** -0.5 if scale is None else scale, num_ctas, None, 0,
+        sp[0], sp[1], P, pages[0], block_table.data_ptr(), block_table.stride(0), q_pos.data_ptr(),
+        None if q_lens is None else q_lens.data_ptr(), shape[0], shape[1], shape[2], pages[1],
+        HEAD_DIM, max_kv_len, _SCALE if scale is None else scale, num_ctas, None, 0,
         _lib.DECODE_STABLE_PREFIX if stable_prefix else 0)
 
 
+_SCALE = HEAD_DIM ** -0.5
+
+
 def decode_into(q, kv_pages, block_table, q_pos, out, workspace, max_kv_len: int,
-                scale: float | None, q_lens, num_ctas: int, stable_prefix: bool) -> None:
+                scale: float | None = None, q_lens=None, num_ctas: int = 0,
+                stable_prefix: bool = False) -> None:
     """``out = attention(q, 4-bit pages)``: the body of ``solort_attn::gqa_decode_paged_int4``. A short
     or misaligned workspace is the library's SOLORT_ERR_WORKSPACE, raised as ``RuntimeError``."""
     index, a = decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len, scale, q_lens, num_ctas,
                            stable_prefix)
-    if workspace.numel():
-        _need(workspace.device == q.device, f"workspace is on {workspace.device}, not on {q.device}")
+    n = workspace.numel()
+    if n:
+        _need(workspace.get_device() == index, f"workspace is on {workspace.device}, not on {q.device}")
         _need(workspace.is_contiguous(), "workspace must be contiguous")
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), n * workspace.element_size()
     if q.numel():
         _launch("solort_attn_decode_int4", a, index)
 

@@ -46,22 +46,6 @@ __device__ __forceinline__ void pdl_launch_dependents() {
 __device__ __forceinline__ float lo_bf16(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-  v[0] = lo_bf16(u.x);
-  v[1] = hi_bf16(u.x);
-  v[2] = lo_bf16(u.y);
-  v[3] = hi_bf16(u.y);
-  v[4] = lo_bf16(u.z);
-  v[5] = hi_bf16(u.z);
-  v[6] = lo_bf16(u.w);
-  v[7] = hi_bf16(u.w);
-}
-
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
-}
-
 // Byte offset of slot row `token` of KV head `head` (its 8-token block) in an arena.
 __device__ __forceinline__ int64_t block_offset(int64_t page, int row, int head, int64_t page_stride,
                                                 int64_t head_stride) {
@@ -69,77 +53,207 @@ __device__ __forceinline__ int64_t block_offset(int64_t page, int row, int head,
          static_cast<int64_t>(row / kBlockTokens) * kBlockBytes;
 }
 
-// Codes (nibble j = x[j]) and packed scale / mid of one group of 32 values held by four adjacent
-// lanes, eight each. Every step is an IEEE fp32 operation in a fixed order, without contraction, so
-// a value next to the border of two codes falls on the same side wherever the formula is evaluated
-// in fp32; the quotients are true divisions, for which exact halves stay exact halves. A group with
-// an infinity or a NaN reads back as NaN throughout: a broken input stays visible.
+// Pairs of fp32 (the packed instructions take half the issue slots). The compiler contracts a packed
+// product and a packed sum of it.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 dup(float a) { return pair(a, a); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN goes on
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// a / b, correctly rounded, from y = 1 / b, correctly rounded: Markstein's correction (IBM J. Res. Dev.
+// 34(1), 1990). With q = a y and r = a - q b, exact in an fma, the quotient is q + r y as long as
+// nothing underflows.
+__device__ __forceinline__ f2 quotient2(f2 a, f2 minus_b, f2 y) {
+  const f2 q = mul2(a, y);
+  return fma2(fma2(q, minus_b, a), y, q);
+}
+
+// The scale and mid of a group of 32 values from its least and greatest, and the codes of its pairs.
+//
+// Every step is an IEEE fp32 operation in a fixed order, without contraction, so a value next to the
+// border of two codes falls on the same side wherever the formula is evaluated in fp32; quotients
+// are correctly rounded, so that exact halves stay exact halves. A group with an infinity or a NaN
+// (lo, hi: with NaN going on) reads back as NaN throughout: a broken input stays visible.
+//
+// The quotients by the step are quotient2's, its reciprocal from the hardware's approximation and one
+// Newton step (correctly rounded for every bf16 step); a step outside 2^+-90 takes true divisions. No
+// code needs clamping: step >= need (1 - 2^-23), so that d / step lies within 7.5 (1 + 2^-22) and its
+// sum with 7.5 rounds to 0..15.
+struct Quantiser {
+  f2 m2, s2, y2;
+  float step;
+  uint32_t meta;
+  bool plain;
+
+  __device__ __forceinline__ Quantiser(float lo, float hi) {
+    const float mid = __bfloat162float(
+        __float2bfloat16_rn(__fadd_rn(__fmul_rn(0.5f, lo), __fmul_rn(0.5f, hi))));
+    const float wide = max_nan(__fsub_rn(hi, mid), __fsub_rn(mid, lo));
+    plain = wide >= 0x1p-86f && wide <= 0x1p90f;
+    constexpr float kSeventh = 1.f / 7.5f;
+    const float n0 = __fmul_rn(wide, kSeventh);
+    float need = fmaf(fmaf(-n0, 7.5f, wide), kSeventh, n0);
+    if (__builtin_expect(!plain, 0)) need = __fdiv_rn(wide, 7.5f);
+    const uint32_t sbits = (__float_as_uint(need) + 0xffffu) & 0xffff0000u;  // need >= 0
+    step = sbits ? __uint_as_float(sbits) : 1.f;
+    float y0;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(step));
+    m2 = dup(-mid);
+    s2 = dup(-step);
+    y2 = dup(fmaf(fmaf(-step, y0, 1.f), y0, y0));
+    meta = wide < INFINITY ? __byte_perm(sbits, __float_as_uint(mid), 0x7632) : 0x7fff7fffu;
+  }
+  // The word of eight codes, nibble j = value j. Rounded to an integer, ties to even, by a sum with
+  // 1.5 2^23, whose bits add up to one constant for the eight.
+  __device__ __forceinline__ uint32_t codes(const f2 (&x)[4]) const {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const f2 d = add2(x[i], m2);
+      f2 q;
+      if (__builtin_expect(plain, 1)) {
+        q = quotient2(d, s2, y2);
+      } else {
+        const float2 v = both(d);
+        q = pair(__fdiv_rn(v.x, step), __fdiv_rn(v.y, step));
+      }
+      const float2 r = both(add2(add2(q, dup(7.5f)), dup(12582912.f)));
+      w = (w << 4) + __float_as_uint(r.y);
+      w = (w << 4) + __float_as_uint(r.x);
+    }
+    return w - 0x4b400000u * 0x11111111u;
+  }
+};
+
+__device__ __forceinline__ void unpack_pairs(const uint4& u, f2 (&x)[4]) {
+  x[0] = pair(lo_bf16(u.x), hi_bf16(u.x));
+  x[1] = pair(lo_bf16(u.y), hi_bf16(u.y));
+  x[2] = pair(lo_bf16(u.z), hi_bf16(u.z));
+  x[3] = pair(lo_bf16(u.w), hi_bf16(u.w));
+}
+__device__ __forceinline__ uint4 pack_pairs(const f2 (&x)[4]) {
+  const float2 a = both(x[0]), b = both(x[1]), c = both(x[2]), d = both(x[3]);
+  return make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y), pack_bf16x2(c.x, c.y), pack_bf16x2(d.x, d.y));
+}
+
+// A group of fp32 values held by four adjacent lanes, eight each: this lane's codes, and the group's
+// scale and mid.
 struct Group {
   uint32_t codes, meta;
 };
-__device__ __forceinline__ Group quantise8(const float (&x)[8], unsigned mask) {
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+__device__ __forceinline__ Group quantise8(const f2 (&x)[4], unsigned mask) {
+  float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = both(x[i]);
+    lo = min_nan(lo, min_nan(v.x, v.y));
+    hi = max_nan(hi, max_nan(v.x, v.y));
   }
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(mask, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(mask, hi, o));
   }
-  const unsigned quad = 0xfu << (threadIdx.x & 28);
-  bad = (__ballot_sync(mask, bad) & quad) != 0;
-  const float mid = __bfloat162float(
-      __float2bfloat16_rn(__fadd_rn(__fmul_rn(0.5f, lo), __fmul_rn(0.5f, hi))));
-  const float need = __fdiv_rn(fmaxf(__fsub_rn(hi, mid), __fsub_rn(mid, lo)), 7.5f);
-  const uint32_t sbits = (__float_as_uint(need) + 0xffffu) & 0xffff0000u;  // need >= 0
-  const float step = sbits ? __uint_as_float(sbits) : 1.f;
-  Group g;
-  g.codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = __float2int_rn(__fadd_rn(__fdiv_rn(__fsub_rn(x[i], mid), step), 7.5f));
-    g.codes |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * i);
-  }
-  g.meta = bad ? 0x7fff7fffu : (sbits >> 16) | (__float_as_uint(mid) & 0xffff0000u);
-  return g;
+  const Quantiser q(lo, hi);
+  return {q.codes(x), q.meta};
 }
 
-// Write one row, held by eight adjacent lanes (lane l8: dims 8 l8.. as `a`, 64 + 8 l8.. as `b`), to
-// row i of the block at `blk`.
-__device__ __forceinline__ void store_row(uint8_t* blk, int i, int l8, bool is_value, const Group& a,
-                                          const Group& b) {
-  const int t = l8 & 3, g = l8 >> 2;  // `a` is group g, `b` group g + 2
-  if (is_value) {
-    uint8_t* pair = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
+// A group of 32 bf16 values in one lane: its codes (word w: values 8 w .. 8 w + 7), scale and mid.
+__device__ __forceinline__ uint32_t quantise32(const uint4 (&u)[4], uint32_t (&codes)[4]) {
+  __nv_bfloat162 lo, hi;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint8_t* unit = pair + 16 * ((2 * t + h) ^ (i & 6));  // place u ^ 2p, p = i / 2
-      *reinterpret_cast<uint16_t*>(unit) = static_cast<uint16_t>(a.codes >> (16 * h));
-      *reinterpret_cast<uint16_t*>(unit + 8) = static_cast<uint16_t>(b.codes >> (16 * h));
-    }
-  } else {
-    uint32_t* chunk = reinterpret_cast<uint32_t*>(blk + 64 * i + 16 * t);
-    chunk[g] = a.codes;
-    chunk[g + 2] = b.codes;
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[i]);
+    const __nv_bfloat162 l = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+    const __nv_bfloat162 g = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    lo = i ? __hmin2_nan(lo, l) : l;
+    hi = i ? __hmax2_nan(hi, g) : g;
   }
+  const Quantiser q(min_nan(__low2float(lo), __high2float(lo)), max_nan(__low2float(hi), __high2float(hi)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f2 x[4];
+    unpack_pairs(u[i], x);
+    codes[i] = q.codes(x);
+  }
+  return q.meta;
+}
+
+// Write one key row, held by eight adjacent lanes (lane l8: dims 8 l8.. as `a`, 64 + 8 l8.. as `b`),
+// to row i of the block at `blk`.
+__device__ __forceinline__ void store_key(uint8_t* blk, int i, int l8, const Group& a, const Group& b) {
+  const int t = l8 & 3, g = l8 >> 2;  // `a` is of group g, `b` of group g + 2
+  uint32_t* chunk = reinterpret_cast<uint32_t*>(blk + 64 * i + 16 * t);
+  chunk[g] = a.codes;
+  chunk[g + 2] = b.codes;
   if (t == 0) {
-    uint32_t* m = reinterpret_cast<uint32_t*>(blk + (is_value ? kOffVScale : kOffKScale) + 16 * i);
+    uint32_t* m = reinterpret_cast<uint32_t*>(blk + kOffKScale + 16 * i);
     m[g] = a.meta;
     m[g + 2] = b.meta;
   }
 }
-
-// The values of eight codes: mid + scale * (code - 7.5); the product is exact in fp32.
-__device__ __forceinline__ void held8(uint32_t codes, uint32_t meta, float (&x)[8]) {
-  const float s = lo_bf16(meta), mid = hi_bf16(meta);
+// Write group g of a row, held by one lane.
+__device__ __forceinline__ void store_group(uint8_t* blk, int i, int g, bool is_value, const uint32_t (&codes)[4],
+                                            uint32_t meta) {
+  if (is_value) {
+    uint8_t* values = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    x[i] = fmaf(s, static_cast<float>((codes >> (4 * i)) & 15u) - 7.5f, mid);
+    for (int u = 0; u < 8; ++u)  // place u ^ 2p, p = i / 2
+      *reinterpret_cast<uint16_t*>(values + 16 * (u ^ (i & 6))) = static_cast<uint16_t>(codes[u >> 1] >> (16 * (u & 1)));
+  } else {
+    uint32_t* keys = reinterpret_cast<uint32_t*>(blk + 64 * i) + g;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) keys[4 * t] = codes[t];
+  }
+  reinterpret_cast<uint32_t*>(blk + (is_value ? kOffVScale : kOffKScale) + 16 * i)[g] = meta;
+}
+
+// The values of eight codes as bf16: mid + scale (code - 7.5), whose product is exact in fp32. A code
+// one bit up in the low bits of 2^22 is the float 2^22 + code.
+__device__ __forceinline__ uint4 held8(uint32_t codes, uint32_t meta) {
+  const f2 s = dup(lo_bf16(meta)), mid = dup(hi_bf16(meta)), centre = dup(-4194311.5f);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = i ? codes >> (8 * i - 1) : codes << 1, b = codes >> (8 * i + 3);
+    const f2 c = add2(pair(__uint_as_float(a & 0x1eu | 0x4a800000u), __uint_as_float(b & 0x1eu | 0x4a800000u)), centre);
+    const float2 v = both(fma2(s, c, mid));
+    o[i] = pack_bf16x2(v.x, v.y);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 }  // namespace i4

@@ -7,11 +7,16 @@
 // token, so one launch serves a batch of sequences, where the reference runs one at a time.
 // store_kernel: the codes of given K / V rows. load_kernel: the values of given slots as bf16 rows.
 //
-// Eight lanes hold a row of 128 dims: lane l takes dims 8l..8l+7 and 64 + 8l..64 + 8l+7, two 16-byte
-// accesses, and so both members of its rotate-half pairs; a quantisation group of 32 is four
-// adjacent lanes. A warp works on four rows.
+// Where a row is rotated, eight lanes hold its 128 dims: lane l takes dims 8l..8l+7 and 64 + 8l..64 +
+// 8l+7, two 16-byte accesses, and so both members of its rotate-half pairs; a quantisation group of 32
+// is four adjacent lanes. Where it is only quantised, four lanes hold it, a group each: what a group
+// costs once (its scale, mid and reciprocal) is then paid for 32 values instead of 8, and nothing is
+// exchanged. A CTA works on tokens of one head, which share the cache lines that they write; the
+// append's query CTAs go over several heads, with the tokens' RoPE rows in registers.
 //
-// All three are bound by the bytes they move, and for a decode step by their launch.
+// All three are bound by the bytes they move, and for a decode step by their launch. 8 KV heads:
+// storing 16380 rows MEASURE_STORE, loading 32001 rows MEASURE_LOAD; appending a prompt of 8190
+// tokens with 32 query heads MEASURE_APPEND.
 #include <math.h>
 
 #include "host_util.h"
@@ -25,6 +30,8 @@ namespace i4 {
 
 constexpr int kRowThreads = 128;
 constexpr int kRowsPerCta = kRowThreads / 8;
+constexpr int kGroupRowsPerCta = kRowThreads / 4;  // of four lanes a row
+constexpr int kFullCtas = 16;  // CTAs per SM from which a CTA takes more than one round of rows
 
 struct Arena {
   uint8_t* base;
@@ -43,6 +50,7 @@ struct AppendParams {
   const bf16* qkv;
   int64_t qkv_st;
   int t, nh, nkv;
+  int q_heads, q_ctas;  // query heads of a CTA, and CTAs along the query heads
   const bf16* qn;
   const bf16* kn;
   float eps;
@@ -57,77 +65,123 @@ struct AppendParams {
   Arena ar;
 };
 
+__device__ __forceinline__ f2 sum_of_products(f2 a, f2 b, f2 c, f2 d) {
+  const float2 x = both(a), y = both(b), u = both(c), v = both(d);
+  return pair(__fadd_rn(__fmul_rn(x.x, y.x), __fmul_rn(u.x, v.x)),
+              __fadd_rn(__fmul_rn(x.y, y.y), __fmul_rn(u.y, v.y)));
+}
+
 // The norm's sum of squares is fp32 for queries, which are rounded to bf16 at the end, and fp64 for
 // keys: a key's last fp32 bit can decide between two codes, and with the sum all but exact its value
-// does not depend on the order of the sum. Norm and rotation stay in fp32 with one rounding at the
-// end (the bf16 cache's prologue rounds after each step, as the reference's torch ops do).
-__global__ void __launch_bounds__(kRowThreads) append_kernel(const AppendParams p) {
+// does not depend on the order of the sum; its products and sums are each rounded on their own, without
+// contraction. Norm and rotation stay in fp32 with one rounding at the end (the bf16 cache's prologue
+// rounds after each step, as the reference's torch ops do).
+// True if `slot` (and `pos`) name a row; a bad one is reported.
+__device__ __forceinline__ bool row_there(long long slot, const Arena& ar, bool report, bool pos_ok = true) {
+  if (slot == -1) return false;
+  if (slot >= 0 && slot < ar.slots && pos_ok) return true;
+  if (report) atomicOr(&g_int4_rows_status, kDevErrSlot);
+  return false;
+}
+
+// Grid: (tokens, [query heads, q_heads each | key heads | value heads]).
+__global__ void __launch_bounds__(kRowThreads, 6) append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l8 = lane & 7;
-  const unsigned mask = 0xffu << (lane & 24);
-  const int heads = p.nh + 2 * p.nkv;
-  const int row = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);
-  if (row >= p.t * heads) return;
-  const int tok = row / heads, head = row - tok * heads;
-  const long long slot = p.slots[tok], pos = p.positions[tok];
-  if (slot == -1) return;
-  if (slot < 0 || slot >= p.ar.slots || pos < 0 || pos >= p.rope_rows) {
-    if (l8 == 0) atomicOr(&g_int4_rows_status, kDevErrSlot);
+  const int y = blockIdx.y;
+  if (y >= p.q_ctas + p.nkv) {  // values: four lanes a row, two rounds of tokens
+    const int head = y - p.q_ctas - p.nkv, g = threadIdx.x & 3;
+    if (threadIdx.x >= kRowThreads / 2) return;
+    const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 2);
+    if (tok >= p.t) return;
+    const long long slot = p.slots[tok], pos = p.positions[tok];
+    if (!row_there(slot, p.ar, g == 0, pos >= 0 && pos < p.rope_rows)) return;
+    const uint4* src = reinterpret_cast<const uint4*>(
+        p.qkv + tok * p.qkv_st + static_cast<int64_t>(p.nh + p.nkv + head) * kHD + g * 32);
+    const uint4 u[4] = {src[0], src[1], src[2], src[3]};
+    uint32_t codes[4];
+    const uint32_t meta = quantise32(u, codes);
+    store_group(slot_block(p.ar, slot, head), static_cast<int>(slot) & 7, g, true, codes, meta);
     return;
   }
-  const bf16* src = p.qkv + tok * p.qkv_st + head * kHD + l8 * 8;
-  float a[8], b[8];
-  unpack8(*reinterpret_cast<const uint4*>(src), a);
-  unpack8(*reinterpret_cast<const uint4*>(src + 64), b);
-  const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-  if (!is_v) {
-    float r;
-    if (is_q) {
-      float ss = 0.f;
+  const int l8 = threadIdx.x & 7;
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
+  const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);
+  if (tok >= p.t) return;
+  const long long slot = p.slots[tok], pos = p.positions[tok];
+  if (!row_there(slot, p.ar, l8 == 0, pos >= 0 && pos < p.rope_rows)) return;
+  const bool is_q = y < p.q_ctas;
+  const int first = is_q ? y * p.q_heads : p.nh + y - p.q_ctas;
+  const int last = is_q ? min(first + p.q_heads, p.nh) : first + 1;
+  const bf16* src = p.qkv + tok * p.qkv_st + l8 * 8;
+  uint4 ua = *reinterpret_cast<const uint4*>(src + first * kHD);
+  uint4 ub = *reinterpret_cast<const uint4*>(src + first * kHD + 64);
+  f2 ca[4], cb[4], sa[4], sb[4], wa[4], wb[4];
+  const int64_t ro = pos * p.rope_st + l8 * 8;
+  const bf16* w = (is_q ? p.qn : p.kn) + l8 * 8;
+  unpack_pairs(*reinterpret_cast<const uint4*>(p.cos + ro), ca);
+  unpack_pairs(*reinterpret_cast<const uint4*>(p.cos + ro + 64), cb);
+  unpack_pairs(*reinterpret_cast<const uint4*>(p.sin + ro), sa);
+  unpack_pairs(*reinterpret_cast<const uint4*>(p.sin + ro + 64), sb);
+  unpack_pairs(*reinterpret_cast<const uint4*>(w), wa);
+  unpack_pairs(*reinterpret_cast<const uint4*>(w + 64), wb);
+  constexpr f2 kMinus = 0x8000000080000000ull;
+  f2 a[4], b[4];
+  if (!is_q) {
+    unpack_pairs(ua, a);
+    unpack_pairs(ub, b);
+    double ss = 0.;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      r = rsqrtf(ss * (1.f / kHD) + p.eps);
-    } else {
-      double ss = 0.;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)  // products of bf16 values are exact in fp32
-        ss += static_cast<double>(a[i] * a[i]) + static_cast<double>(b[i] * b[i]);
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      r = static_cast<float>(rsqrt(ss * (1. / kHD) + static_cast<double>(p.eps)));
+    for (int i = 0; i < 4; ++i) {  // squares of bf16 values are exact in fp32
+      const float2 x = both(mul2(a[i], a[i])), z = both(mul2(b[i], b[i]));
+      ss += static_cast<double>(x.x) + static_cast<double>(x.y);
+      ss += static_cast<double>(z.x) + static_cast<double>(z.y);
     }
-    const bf16* wp = (is_q ? p.qn : p.kn) + l8 * 8;
-    const int64_t ro = pos * p.rope_st + l8 * 8;
-    float w[8], ca[8], cb[8], sa[8], sb[8];
-    unpack8(*reinterpret_cast<const uint4*>(wp), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = __fmul_rn(__fmul_rn(a[i], r), w[i]);
-    unpack8(*reinterpret_cast<const uint4*>(wp + 64), w);
+    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    const f2 r = dup(static_cast<float>(rsqrt(ss * (1. / kHD) + static_cast<double>(p.eps))));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __fmul_rn(__fmul_rn(b[i], r), w[i]);
-    unpack8(*reinterpret_cast<const uint4*>(p.cos + ro), ca);
-    unpack8(*reinterpret_cast<const uint4*>(p.cos + ro + 64), cb);
-    unpack8(*reinterpret_cast<const uint4*>(p.sin + ro), sa);
-    unpack8(*reinterpret_cast<const uint4*>(p.sin + ro + 64), sb);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = __fadd_rn(__fmul_rn(x, ca[i]), __fmul_rn(-y, sa[i]));
-      b[i] = __fadd_rn(__fmul_rn(y, cb[i]), __fmul_rn(x, sb[i]));
+    for (int i = 0; i < 4; ++i) {  // not packed: the compiler contracts packed products and sums
+      const f2 x = mul2(mul2(a[i], r), wa[i]), z = mul2(mul2(b[i], r), wb[i]);
+      a[i] = sum_of_products(x, ca[i], z, sa[i] ^ kMinus);
+      b[i] = sum_of_products(z, cb[i], x, sb[i]);
     }
-    if (is_q) {
-      bf16* o = p.q_out + tok * p.qo_st + head * p.qo_sh + l8 * 8;
-      *reinterpret_cast<uint4*>(o) = pack8(a);
-      *reinterpret_cast<uint4*>(o + 64) = pack8(b);
-      return;
-    }
+    const Group ga = quantise8(a, mask), gb = quantise8(b, mask);
+    store_key(slot_block(p.ar, slot, y - p.q_ctas), static_cast<int>(slot) & 7, l8, ga, gb);
+    return;
   }
-  uint8_t* blk = slot_block(p.ar, slot, head - p.nh - (is_v ? p.nkv : 0));
-  const Group ga = quantise8(a, mask), gb = quantise8(b, mask);
-  store_row(blk, static_cast<int>(slot) & 7, l8, is_v, ga, gb);
+  // out = r (x w cos + partner w sin): the weights join the tables once for all heads.
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ca[i] = mul2(ca[i], wa[i]);
+    cb[i] = mul2(cb[i], wb[i]);
+    sa[i] = mul2(sa[i], wb[i]) ^ kMinus;
+    sb[i] = mul2(sb[i], wa[i]);
+  }
+  bf16* to = p.q_out + tok * p.qo_st + l8 * 8;
+  for (int head = first; head < last; ++head) {
+    unpack_pairs(ua, a);
+    unpack_pairs(ub, b);
+    if (head + 1 < last) {
+      ua = *reinterpret_cast<const uint4*>(src + (head + 1) * kHD);
+      ub = *reinterpret_cast<const uint4*>(src + (head + 1) * kHD + 64);
+    }
+    f2 sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fma2(a[i], a[i], fma2(b[i], b[i], sum));
+    float ss = both(sum).x + both(sum).y;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    const f2 r = dup(rsqrtf(ss * (1.f / kHD) + p.eps));
+    f2 x[4], z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = mul2(fma2(a[i], ca[i], mul2(b[i], sa[i])), r);
+      z[i] = mul2(fma2(b[i], cb[i], mul2(a[i], sb[i])), r);
+    }
+    *reinterpret_cast<uint4*>(to + head * p.qo_sh) = pack_pairs(x);
+    *reinterpret_cast<uint4*>(to + head * p.qo_sh + 64) = pack_pairs(z);
+  }
 }
 
 struct StoreParams {
@@ -142,26 +196,28 @@ struct StoreParams {
 __global__ void __launch_bounds__(kRowThreads) store_kernel(const StoreParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l8 = lane & 7;
-  const unsigned mask = 0xffu << (lane & 24);
-  const int row = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);  // (token, K or V, head)
-  if (row >= p.t * p.nkv * 2) return;
-  const int tok = row / (2 * p.nkv), rem = row - tok * 2 * p.nkv;
-  const bool is_v = rem >= p.nkv;
-  const int head = is_v ? rem - p.nkv : rem;
-  const long long slot = p.slots[tok];
-  if (slot == -1) return;
-  if (slot < 0 || slot >= p.ar.slots) {
-    if (l8 == 0) atomicOr(&g_int4_rows_status, kDevErrSlot);
-    return;
+  const int g = threadIdx.x & 3;
+  const bool is_v = static_cast<int>(blockIdx.y) >= p.nkv;  // K heads, then V heads
+  const int head = blockIdx.y - (is_v ? p.nkv : 0);
+  const bf16* src = (is_v ? p.value + head * p.v_sh : p.key + head * p.k_sh) + g * 32;
+  const int64_t st = is_v ? p.v_st : p.k_st;
+  const int step = gridDim.x * kGroupRowsPerCta;
+  int tok = blockIdx.x * kGroupRowsPerCta + (threadIdx.x >> 2);
+  uint4 u[4];
+  if (tok < p.t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = reinterpret_cast<const uint4*>(src + tok * st)[i];
+  for (; tok < p.t; tok += step) {
+    const long long slot = p.slots[tok];
+    const uint4 v[4] = {u[0], u[1], u[2], u[3]};
+    if (tok + step < p.t)  // the next round's rows
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = reinterpret_cast<const uint4*>(src + (tok + step) * st)[i];
+    if (!row_there(slot, p.ar, g == 0)) continue;
+    uint32_t codes[4];
+    const uint32_t meta = quantise32(v, codes);
+    store_group(slot_block(p.ar, slot, head), static_cast<int>(slot) & 7, g, is_v, codes, meta);
   }
-  const bf16* src = (is_v ? p.value + tok * p.v_st + head * p.v_sh
-                          : p.key + tok * p.k_st + head * p.k_sh) + l8 * 8;
-  float a[8], b[8];
-  unpack8(*reinterpret_cast<const uint4*>(src), a);
-  unpack8(*reinterpret_cast<const uint4*>(src + 64), b);
-  const Group ga = quantise8(a, mask), gb = quantise8(b, mask);
-  store_row(slot_block(p.ar, slot, head), static_cast<int>(slot) & 7, l8, is_v, ga, gb);
 }
 
 struct LoadParams {
@@ -176,40 +232,32 @@ struct LoadParams {
 __global__ void __launch_bounds__(kRowThreads) load_kernel(const LoadParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int l8 = threadIdx.x & 7;
-  const int row = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);  // (head, token)
-  if (row >= p.t * p.nkv) return;
-  const int head = row / p.t, tok = row - head * p.t;
-  const long long slot = p.slots[tok];
-  if (slot == -1) return;
-  if (slot < 0 || slot >= p.ar.slots) {
-    if (l8 == 0) atomicOr(&g_int4_rows_status, kDevErrSlot);
-    return;
-  }
-  const uint8_t* blk = slot_block(p.ar, slot, head);
-  const int i = static_cast<int>(slot) & 7, t = l8 & 3, g = l8 >> 2;
-  const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + 64 * i + 16 * t);
-  const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + kOffKScale + 16 * i);
-  const uint32_t* vm = reinterpret_cast<const uint32_t*>(blk + kOffVScale + 16 * i);
-  const uint8_t* pair = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
-  uint32_t va = 0, vb = 0;
+  const int l8 = threadIdx.x & 7, t = l8 & 3, g = l8 >> 2;
+  const int head = blockIdx.y;
+  for (int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3); tok < p.t; tok += gridDim.x * kRowsPerCta) {
+    const long long slot = p.slots[tok];
+    if (!row_there(slot, p.ar, l8 == 0)) continue;
+    const uint8_t* blk = slot_block(p.ar, slot, head);
+    const int i = static_cast<int>(slot) & 7;
+    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + 64 * i + 16 * t);
+    const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + kOffKScale + 16 * i);
+    const uint32_t* vm = reinterpret_cast<const uint32_t*>(blk + kOffVScale + 16 * i);
+    const uint8_t* values = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
+    uint32_t va = 0, vb = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint8_t* unit = pair + 16 * ((2 * t + h) ^ (i & 6));
-    va |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit)) << (16 * h);
-    vb |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit + 8)) << (16 * h);
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* unit = values + 16 * ((2 * t + h) ^ (i & 6));
+      va |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit)) << (16 * h);
+      vb |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit + 8)) << (16 * h);
+    }
+    const uint32_t ka = kc[g], kb = kc[g + 2], kma = km[g], kmb = km[g + 2], vma = vm[g], vmb = vm[g + 2];
+    bf16* k = p.key + tok * p.k_st + head * p.k_sh + l8 * 8;
+    *reinterpret_cast<uint4*>(k) = held8(ka, kma);
+    *reinterpret_cast<uint4*>(k + 64) = held8(kb, kmb);
+    bf16* v = p.value + tok * p.v_st + head * p.v_sh + l8 * 8;
+    *reinterpret_cast<uint4*>(v) = held8(va, vma);
+    *reinterpret_cast<uint4*>(v + 64) = held8(vb, vmb);
   }
-  float x[8];
-  bf16* k = p.key + tok * p.k_st + head * p.k_sh + l8 * 8;
-  held8(kc[g], km[g], x);
-  *reinterpret_cast<uint4*>(k) = pack8(x);
-  held8(kc[g + 2], km[g + 2], x);
-  *reinterpret_cast<uint4*>(k + 64) = pack8(x);
-  bf16* v = p.value + tok * p.v_st + head * p.v_sh + l8 * 8;
-  held8(va, vm[g], x);
-  *reinterpret_cast<uint4*>(v) = pack8(x);
-  held8(vb, vm[g + 2], x);
-  *reinterpret_cast<uint4*>(v + 64) = pack8(x);
 }
 
 // Checks shared by the three entry points: the arena and the slots.
@@ -235,10 +283,10 @@ int make_arena(const void* pages, int64_t page_stride, int64_t head_stride, int3
 }
 
 template <typename P>
-int launch_rows(void (*kernel)(const P), const P& prm, int64_t rows, void* stream) {
-  if (rows > (1ll << 30)) return SOLORT_ERR_UNSUPPORTED;
+int launch_rows(void (*kernel)(const P), const P& prm, int64_t x, int64_t y, void* stream) {
+  if (x > (1ll << 30) || y > 65535) return SOLORT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + kRowsPerCta - 1) / kRowsPerCta));
+  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
   cfg.blockDim = dim3(kRowThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute at[1];
@@ -248,6 +296,14 @@ int launch_rows(void (*kernel)(const P), const P& prm, int64_t rows, void* strea
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kernel, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   return launch_status();
+}
+
+// CTAs along the tokens, `rows` each, for a grid with `y` heads; fewer, with several rounds each, where
+// that would give over kFullCtas per SM.
+inline int64_t token_ctas(int tokens, int rows, int64_t y, const DeviceInfo& di) {
+  const int64_t all = (static_cast<int64_t>(tokens) + rows - 1) / rows;
+  const int64_t cap = static_cast<int64_t>(di.sm_count) * kFullCtas / y;
+  return all < cap || cap < 1 ? (cap < 1 ? 1 : all) : cap;
 }
 
 }  // namespace i4
@@ -302,9 +358,12 @@ extern "C" int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* 
   p.q_out = static_cast<bf16*>(a->q_out);
   p.qo_st = a->q_out_stride_token;
   p.qo_sh = a->q_out_stride_head;
-  const int64_t rows =
-      static_cast<int64_t>(a->num_tokens) * (static_cast<int64_t>(a->num_qo_heads) + 2ll * a->num_kv_heads);
-  return i4::launch_rows(i4::append_kernel, p, rows, stream);
+  // One query head per CTA while the GPU is not full, and up to eight.
+  const int64_t x = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta;
+  const int64_t per = x * a->num_qo_heads / (static_cast<int64_t>(di.sm_count) * i4::kFullCtas);
+  p.q_heads = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
+  p.q_ctas = (a->num_qo_heads + p.q_heads - 1) / p.q_heads;
+  return i4::launch_rows(i4::append_kernel, p, x, p.q_ctas + 2ll * a->num_kv_heads, stream);
 }
 
 extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* stream) {
@@ -331,7 +390,9 @@ extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* str
   p.t = a->num_tokens;
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
-  return i4::launch_rows(i4::store_kernel, p, 2ll * a->num_tokens * a->num_kv_heads, stream);
+  const int64_t y = 2ll * a->num_kv_heads;
+  return i4::launch_rows(i4::store_kernel, p, i4::token_ctas(a->num_tokens, i4::kGroupRowsPerCta, y, di), y,
+                         stream);
 }
 
 extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* stream) {
@@ -358,6 +419,6 @@ extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* strea
   p.t = a->num_tokens;
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
-  return i4::launch_rows(i4::load_kernel, p, static_cast<int64_t>(a->num_tokens) * a->num_kv_heads,
-                         stream);
+  return i4::launch_rows(i4::load_kernel, p, i4::token_ctas(a->num_tokens, i4::kRowsPerCta, a->num_kv_heads, di),
+                         a->num_kv_heads, stream);
 }

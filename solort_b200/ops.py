@@ -545,6 +545,14 @@ def kv_store(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
 
 
 # ---- the paged KV cache held in 4 bits ----
+#
+# A decode step makes these calls once a layer, some of them shorter on the GPU than the dispatcher's
+# way round to them (about 3 us a call): on plain tensors outside a trace they go to the ops' body
+# directly.
+
+def _plain(t: torch.Tensor) -> bool:
+    return type(t) is torch.Tensor and t.is_cuda and not torch.compiler.is_compiling()
+
 
 def kv_pages_int4(num_pages: int, num_kv_heads: int, page_size: int,
                   device: torch.device | str = "cuda") -> torch.Tensor:
@@ -564,7 +572,7 @@ def kv_store_int4(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
     """Hold ``key / value [tokens, nkv, 128]`` (bf16; token / head strides multiples of 8) in 4 bits at
     ``slots`` (int64 on the device, ``page * P + row``; -1 skips a row) of ``kv_pages``
     (:func:`kv_pages_int4`; ``torch.ops.solort_attn.kv_store_int4``): the 4-bit :func:`kv_store`."""
-    _OPS.kv_store_int4(key, value, slots, kv_pages)
+    (_calls_int4.store_into if _plain(kv_pages) else _OPS.kv_store_int4)(key, value, slots, kv_pages)
 
 
 def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tensor | None = None,
@@ -577,7 +585,7 @@ def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tens
         key = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
     if value is None:
         value = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
-    _OPS.kv_load_int4(kv_pages, slots, key, value)
+    (_calls_int4.load_into if _plain(kv_pages) else _OPS.kv_load_int4)(kv_pages, slots, key, value)
     return key, value
 
 
@@ -610,8 +618,8 @@ def qk_norm_rope_append_int4(
         q_out = torch.empty(qkv.shape[0], num_qo_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
     elif q_out.dim() != 3 or q_out.shape[1] != num_qo_heads:
         raise RuntimeError(f"q_out must be [tokens, {num_qo_heads}, 128]")
-    _OPS.qk_norm_rope_append_int4(qkv, q_norm_weight, k_norm_weight, float(eps), cos, sin, positions,
-                                  slots, kv_pages, q_out)
+    (_calls_int4.append_into if _plain(kv_pages) else _OPS.qk_norm_rope_append_int4)(
+        qkv, q_norm_weight, k_norm_weight, float(eps), cos, sin, positions, slots, kv_pages, q_out)
     return q_out
 
 
@@ -656,6 +664,7 @@ def gqa_decode_paged_int4(
                                                   a.max_kv_len, a.num_ctas) if q.numel() else 0
         workspace = (torch.empty(need, dtype=torch.uint8, device=q.device) if need
                      else _empty_workspace(q.device))
-    _OPS.gqa_decode_paged_int4(q, kv_pages, block_table, q_pos, out, workspace, int(max_kv_len), scale,
-                               q_lens, int(num_ctas), bool(stable_prefix))
+    (_calls_int4.decode_into if _plain(kv_pages) else _OPS.gqa_decode_paged_int4)(
+        q, kv_pages, block_table, q_pos, out, workspace, int(max_kv_len), scale, q_lens, int(num_ctas),
+        bool(stable_prefix))
     return out

@@ -37,16 +37,10 @@ for _schema in SCHEMAS.values():
     _LIB.define(_schema)
 
 
-def _decode(q, kv_pages, block_table, q_pos, out, workspace, max_kv_len, scale=None, q_lens=None,
-            num_ctas=0, stable_prefix=False):
-    C.decode_into(q, kv_pages, block_table, q_pos, out, workspace, max_kv_len, scale, q_lens, num_ctas,
-                  stable_prefix)
-
-
 _LIB.impl("qk_norm_rope_append_int4", C.append_into, "CUDA")
 _LIB.impl("kv_store_int4", C.store_into, "CUDA")
 _LIB.impl("kv_load_int4", C.load_into, "CUDA")
-_LIB.impl("gqa_decode_paged_int4", _decode, "CUDA")
+_LIB.impl("gqa_decode_paged_int4", C.decode_into, "CUDA")
 
 
 # ---- fake (meta) implementations: the same shape / dtype rules, no data access ----
