@@ -50,7 +50,7 @@ struct AppendParams {
   const bf16* qkv;
   int64_t qkv_st;
   int t, nh, nkv;
-  int q_heads, q_ctas;  // query heads of a CTA, and CTAs along the query heads
+  int heads, q_ctas, kv_ctas;  // heads of a CTA, and CTAs along the query heads and the KV heads
   const bf16* qn;
   const bf16* kn;
   float eps;
@@ -84,24 +84,34 @@ __device__ __forceinline__ bool row_there(long long slot, const Arena& ar, bool 
   return false;
 }
 
-// Grid: (tokens, [query heads, q_heads each | key heads | value heads]).
-__global__ void __launch_bounds__(kRowThreads, 6) append_kernel(const AppendParams p) {
+// Grid: (tokens, [query heads | key heads | value heads], p.heads each).
+__global__ void __launch_bounds__(kRowThreads, 5) append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int y = blockIdx.y;
-  if (y >= p.q_ctas + p.nkv) {  // values: four lanes a row, two rounds of tokens
-    const int head = y - p.q_ctas - p.nkv, g = threadIdx.x & 3;
-    if (threadIdx.x >= kRowThreads / 2) return;
-    const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 2);
+  if (y >= p.q_ctas + p.kv_ctas) {  // values: four lanes a row, two heads at a time
+    const int g = threadIdx.x & 3, first = (y - p.q_ctas - p.kv_ctas) * p.heads;
+    const int last = min(first + p.heads, p.nkv);
+    const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 2 & 15);
     if (tok >= p.t) return;
     const long long slot = p.slots[tok], pos = p.positions[tok];
-    if (!row_there(slot, p.ar, g == 0, pos >= 0 && pos < p.rope_rows)) return;
     const uint4* src = reinterpret_cast<const uint4*>(
-        p.qkv + tok * p.qkv_st + static_cast<int64_t>(p.nh + p.nkv + head) * kHD + g * 32);
-    const uint4 u[4] = {src[0], src[1], src[2], src[3]};
-    uint32_t codes[4];
-    const uint32_t meta = quantise32(u, codes);
-    store_group(slot_block(p.ar, slot, head), static_cast<int>(slot) & 7, g, true, codes, meta);
+        p.qkv + tok * p.qkv_st + static_cast<int64_t>(p.nh + p.nkv) * kHD + g * 32);
+    int head = first + (threadIdx.x >> 6);
+    uint4 u[4];
+    if (head < last)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = src[head * (kHD / 8) + i];
+    if (!row_there(slot, p.ar, g == 0, pos >= 0 && pos < p.rope_rows)) return;
+    for (; head < last; head += 2) {
+      const uint4 v[4] = {u[0], u[1], u[2], u[3]};
+      if (head + 2 < last)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = src[(head + 2) * (kHD / 8) + i];
+      uint32_t codes[4];
+      const uint32_t meta = quantise32(v, codes);
+      store_group(slot_block(p.ar, slot, head), static_cast<int>(slot) & 7, g, true, codes, meta);
+    }
     return;
   }
   const int l8 = threadIdx.x & 7;
@@ -111,8 +121,8 @@ __global__ void __launch_bounds__(kRowThreads, 6) append_kernel(const AppendPara
   const long long slot = p.slots[tok], pos = p.positions[tok];
   if (!row_there(slot, p.ar, l8 == 0, pos >= 0 && pos < p.rope_rows)) return;
   const bool is_q = y < p.q_ctas;
-  const int first = is_q ? y * p.q_heads : p.nh + y - p.q_ctas;
-  const int last = is_q ? min(first + p.q_heads, p.nh) : first + 1;
+  const int first = is_q ? y * p.heads : p.nh + (y - p.q_ctas) * p.heads;
+  const int last = min(first + p.heads, is_q ? p.nh : p.nh + p.nkv);
   const bf16* src = p.qkv + tok * p.qkv_st + l8 * 8;
   uint4 ua = *reinterpret_cast<const uint4*>(src + first * kHD);
   uint4 ub = *reinterpret_cast<const uint4*>(src + first * kHD + 64);
@@ -123,34 +133,42 @@ __global__ void __launch_bounds__(kRowThreads, 6) append_kernel(const AppendPara
   unpack_pairs(*reinterpret_cast<const uint4*>(p.cos + ro + 64), cb);
   unpack_pairs(*reinterpret_cast<const uint4*>(p.sin + ro), sa);
   unpack_pairs(*reinterpret_cast<const uint4*>(p.sin + ro + 64), sb);
-  unpack_pairs(*reinterpret_cast<const uint4*>(w), wa);
-  unpack_pairs(*reinterpret_cast<const uint4*>(w + 64), wb);
   constexpr f2 kMinus = 0x8000000080000000ull;
   f2 a[4], b[4];
   if (!is_q) {
-    unpack_pairs(ua, a);
-    unpack_pairs(ub, b);
-    double ss = 0.;
+    for (int head = first; head < last; ++head) {
+      unpack_pairs(ua, a);
+      unpack_pairs(ub, b);
+      if (head + 1 < last) {
+        ua = *reinterpret_cast<const uint4*>(src + (head + 1) * kHD);
+        ub = *reinterpret_cast<const uint4*>(src + (head + 1) * kHD + 64);
+      }
+      double ss = 0.;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // squares of bf16 values are exact in fp32
-      const float2 x = both(mul2(a[i], a[i])), z = both(mul2(b[i], b[i]));
-      ss += static_cast<double>(x.x) + static_cast<double>(x.y);
-      ss += static_cast<double>(z.x) + static_cast<double>(z.y);
+      for (int i = 0; i < 4; ++i) {  // squares of bf16 values are exact in fp32
+        const float2 x = both(mul2(a[i], a[i])), z = both(mul2(b[i], b[i]));
+        ss += static_cast<double>(x.x) + static_cast<double>(x.y);
+        ss += static_cast<double>(z.x) + static_cast<double>(z.y);
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+      unpack_pairs(*reinterpret_cast<const uint4*>(w), wa);  // of the first-level cache, to save registers
+      unpack_pairs(*reinterpret_cast<const uint4*>(w + 64), wb);
+      const f2 r = dup(static_cast<float>(rsqrt(ss * (1. / kHD) + static_cast<double>(p.eps))));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // not packed: the compiler contracts packed products and sums
+        const f2 x = mul2(mul2(a[i], r), wa[i]), z = mul2(mul2(b[i], r), wb[i]);
+        a[i] = sum_of_products(x, ca[i], z, sa[i] ^ kMinus);
+        b[i] = sum_of_products(z, cb[i], x, sb[i]);
+      }
+      const Group ga = quantise8(a, mask), gb = quantise8(b, mask);
+      store_key(slot_block(p.ar, slot, head - p.nh), static_cast<int>(slot) & 7, l8, ga, gb);
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-    const f2 r = dup(static_cast<float>(rsqrt(ss * (1. / kHD) + static_cast<double>(p.eps))));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // not packed: the compiler contracts packed products and sums
-      const f2 x = mul2(mul2(a[i], r), wa[i]), z = mul2(mul2(b[i], r), wb[i]);
-      a[i] = sum_of_products(x, ca[i], z, sa[i] ^ kMinus);
-      b[i] = sum_of_products(z, cb[i], x, sb[i]);
-    }
-    const Group ga = quantise8(a, mask), gb = quantise8(b, mask);
-    store_key(slot_block(p.ar, slot, y - p.q_ctas), static_cast<int>(slot) & 7, l8, ga, gb);
     return;
   }
   // out = r (x w cos + partner w sin): the weights join the tables once for all heads.
+  unpack_pairs(*reinterpret_cast<const uint4*>(w), wa);
+  unpack_pairs(*reinterpret_cast<const uint4*>(w + 64), wb);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     ca[i] = mul2(ca[i], wa[i]);
@@ -234,30 +252,30 @@ __global__ void __launch_bounds__(kRowThreads) load_kernel(const LoadParams p) {
   pdl_wait();
   const int l8 = threadIdx.x & 7, t = l8 & 3, g = l8 >> 2;
   const int head = blockIdx.y;
-  for (int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3); tok < p.t; tok += gridDim.x * kRowsPerCta) {
-    const long long slot = p.slots[tok];
-    if (!row_there(slot, p.ar, l8 == 0)) continue;
-    const uint8_t* blk = slot_block(p.ar, slot, head);
-    const int i = static_cast<int>(slot) & 7;
-    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + 64 * i + 16 * t);
-    const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + kOffKScale + 16 * i);
-    const uint32_t* vm = reinterpret_cast<const uint32_t*>(blk + kOffVScale + 16 * i);
-    const uint8_t* values = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
-    uint32_t va = 0, vb = 0;
+  const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);
+  if (tok >= p.t) return;
+  const long long slot = p.slots[tok];
+  if (!row_there(slot, p.ar, l8 == 0)) return;
+  const uint8_t* blk = slot_block(p.ar, slot, head);
+  const int i = static_cast<int>(slot) & 7;
+  const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk + 64 * i + 16 * t);
+  const uint32_t* km = reinterpret_cast<const uint32_t*>(blk + kOffKScale + 16 * i);
+  const uint32_t* vm = reinterpret_cast<const uint32_t*>(blk + kOffVScale + 16 * i);
+  const uint8_t* values = blk + kOffV + 128 * (i >> 1) + 4 * g + 2 * (i & 1);
+  uint32_t va = 0, vb = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* unit = values + 16 * ((2 * t + h) ^ (i & 6));
-      va |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit)) << (16 * h);
-      vb |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit + 8)) << (16 * h);
-    }
-    const uint32_t ka = kc[g], kb = kc[g + 2], kma = km[g], kmb = km[g + 2], vma = vm[g], vmb = vm[g + 2];
-    bf16* k = p.key + tok * p.k_st + head * p.k_sh + l8 * 8;
-    *reinterpret_cast<uint4*>(k) = held8(ka, kma);
-    *reinterpret_cast<uint4*>(k + 64) = held8(kb, kmb);
-    bf16* v = p.value + tok * p.v_st + head * p.v_sh + l8 * 8;
-    *reinterpret_cast<uint4*>(v) = held8(va, vma);
-    *reinterpret_cast<uint4*>(v + 64) = held8(vb, vmb);
+  for (int h = 0; h < 2; ++h) {
+    const uint8_t* unit = values + 16 * ((2 * t + h) ^ (i & 6));
+    va |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit)) << (16 * h);
+    vb |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(unit + 8)) << (16 * h);
   }
+  const uint32_t ka = kc[g], kb = kc[g + 2], kma = km[g], kmb = km[g + 2], vma = vm[g], vmb = vm[g + 2];
+  bf16* k = p.key + tok * p.k_st + head * p.k_sh + l8 * 8;
+  *reinterpret_cast<uint4*>(k) = held8(ka, kma);
+  *reinterpret_cast<uint4*>(k + 64) = held8(kb, kmb);
+  bf16* v = p.value + tok * p.v_st + head * p.v_sh + l8 * 8;
+  *reinterpret_cast<uint4*>(v) = held8(va, vma);
+  *reinterpret_cast<uint4*>(v + 64) = held8(vb, vmb);
 }
 
 // Checks shared by the three entry points: the arena and the slots.
@@ -358,12 +376,13 @@ extern "C" int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* 
   p.q_out = static_cast<bf16*>(a->q_out);
   p.qo_st = a->q_out_stride_token;
   p.qo_sh = a->q_out_stride_head;
-  // One query head per CTA while the GPU is not full, and up to eight.
+  // One head per CTA while the GPU is not full, and up to eight.
   const int64_t x = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta;
-  const int64_t per = x * a->num_qo_heads / (static_cast<int64_t>(di.sm_count) * i4::kFullCtas);
-  p.q_heads = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
-  p.q_ctas = (a->num_qo_heads + p.q_heads - 1) / p.q_heads;
-  return i4::launch_rows(i4::append_kernel, p, x, p.q_ctas + 2ll * a->num_kv_heads, stream);
+  const int64_t per = x * (a->num_qo_heads + 2ll * a->num_kv_heads) / (static_cast<int64_t>(di.sm_count) * i4::kFullCtas);
+  p.heads = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
+  p.q_ctas = (a->num_qo_heads + p.heads - 1) / p.heads;
+  p.kv_ctas = (a->num_kv_heads + p.heads - 1) / p.heads;
+  return i4::launch_rows(i4::append_kernel, p, x, p.q_ctas + 2ll * p.kv_ctas, stream);
 }
 
 extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* stream) {
@@ -419,6 +438,6 @@ extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* strea
   p.t = a->num_tokens;
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
-  return i4::launch_rows(i4::load_kernel, p, i4::token_ctas(a->num_tokens, i4::kRowsPerCta, a->num_kv_heads, di),
+  return i4::launch_rows(i4::load_kernel, p, (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta,
                          a->num_kv_heads, stream);
 }
