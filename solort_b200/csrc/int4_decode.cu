@@ -71,7 +71,7 @@ struct Cfg {
   static constexpr int kOffRed = kRing;
   static constexpr int kOffMl = kOffRed + kRed;
   static constexpr int kOffEdge = kOffMl + 2 * kWarps * kRows * 8;
-  static constexpr int kOffRange = kOffEdge + 2 * kWarps * 4;
+  static constexpr int kOffRange = kOffEdge + 2 * kWarps * 24;
   static constexpr int kOffPlaces = (kOffRange + (kWarps + 1) * 12 + 15) / 16 * 16;  // [warp][32 tiles][4]
   static constexpr int kSmem = kOffPlaces + kWarps * 32 * 32;
 };
@@ -333,36 +333,53 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
   raise |= most > 1.f;
   if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
     if (__any_sync(0xffffffffu, most > 1.f)) {
+      // The groups' largest scales, two bf16 bit patterns (not negative: they compare as integers) a word;
+      // a NaN does not count, it makes the sums of the rows that see it NaN by itself.
+      uint32_t top[2];
 #pragma unroll
-      for (int grp = 0; grp < 4; ++grp) {
-        const int q = grp >> 1, e = grp & 1;
-        float mx = 0.f;
+      for (int q = 0; q < 2; ++q) {
+        top[q] = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, lo_bf16(word(meta[i], grp)));
-#pragma unroll
-        for (int o = 1; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float2 old = both(A.sf[q]);
-        const float was = e ? old.y : old.x;
-        if (mx * was > 1.f) {  // the power of two that brings mx into [0.5, 1)
-          const int top = 253 - static_cast<int>(__float_as_uint(mx) >> 23);
-          const float sf = __uint_as_float(static_cast<uint32_t>(max(top, 1)) << 23), f = sf / was;
-          A.sf[q] = e ? pair(old.x, sf) : pair(sf, old.y);
-#pragma unroll
-          for (int c = 0; c < Acc<NT>::kCols; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
-            if (NT > 1)
-              A.xs[c][q & (NT > 1)][2 * e] *= f, A.xs[c][q & (NT > 1)][2 * e + 1] *= f;
-            else
-              A.xs[c][0][2 * q + e] *= f;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = __byte_perm(word(meta[i], 2 * q), word(meta[i], 2 * q + 1), 0x5410);
+          top[q] = __vmaxu2(top[q], two & ~__vcmpgtu2(two, 0x7f7f7f7fu));
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int o = 1; o <= 16; o <<= 1) {
+        const uint32_t t0 = __shfl_xor_sync(0xffffffffu, top[0], o), t1 = __shfl_xor_sync(0xffffffffu, top[1], o);
+        top[0] = __vmaxu2(top[0], t0);
+        top[1] = __vmaxu2(top[1], t1);
+      }
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < 2; ++q) {
+        const float2 was = both(A.sf[q]);
+        float sf[2], f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // The power of two that brings the scale into [0.5, 1).
+          const uint32_t bits = e ? top[q] >> 16 : top[q] & 0xffffu;
+          const float old = e ? was.y : was.x;
+          const float now = __uint_as_float(static_cast<uint32_t>(max(253 - static_cast<int>(bits >> 7), 1)) << 23);
+          sf[e] = bits ? fminf(old, now) : old;
+          f[e] = sf[e] / old;
+        }
+        A.sf[q] = pair(sf[0], sf[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int c = 0; c < Acc<NT>::kCols; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A.o[c][2 * q + e][0][i] *= f[e], A.o[c][2 * q + e][1][i] *= f[e];
+            if (NT > 1)
+              A.xs[c][q & (NT > 1)][2 * e] *= f[e], A.xs[c][q & (NT > 1)][2 * e + 1] *= f[e];
+            else
+              A.xs[c][0][2 * q + e] *= f[e];
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
           sc[i][q] = mul2(pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1))), A.sf[q]);
+      }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -482,6 +499,10 @@ __device__ __forceinline__ float4 chunk_of(const Acc<NT>& A, int nt, int grp, fl
 struct Range {
   int x0, seq, base;
 };
+// A unit of which a warp holds a part: its tiles [u0, u1) of the list, and where its rows belong.
+struct Edge {
+  int u0, u1, seq, head, row0, live;
+};
 
 template <int NT>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
@@ -491,7 +512,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
   // What a warp leaves of a unit that it shares with other warps: its first unit's (begun before the
   // warp's range) in `red`, and its last's (begun in it, going on behind it) where its ring was.
   float2* ml = reinterpret_cast<float2*>(smem + C::kOffMl);   // [2 warp + which][row]
-  int* edge = reinterpret_cast<int*>(smem + C::kOffEdge);     // [2 warp + which]: the unit's first tile, or -1
+  Edge* edge = reinterpret_cast<Edge*>(smem + C::kOffEdge);   // [2 warp + which]; u0 -1: none
   Range* range = reinterpret_cast<Range*>(smem + C::kOffRange);
   auto part_row = [&](int which, int row) {
     return reinterpret_cast<float*>(smem + (which & 1 ? (which >> 1) * kDepth * kTileBytes
@@ -504,7 +525,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
   const uint32_t places = smem_u32(smem) + C::kOffPlaces + warp * 32 * 32;
 
   pdl_launch_dependents();
-  if (lane == 0) edge[2 * warp] = edge[2 * warp + 1] = -1;
+  if (lane == 0) edge[2 * warp].u0 = edge[2 * warp + 1].u0 = -1;
   const bool early = p.stable_prefix != 0;
   if (!early) pdl_wait();
   if (warp == 0) {
@@ -750,8 +771,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       if (!goes_on) span->y = blockIdx.x;
     }
     const int which = 2 * warp + (from_before ? 0 : 1);
-    if ((from_before || goes_on) && lane == 0) edge[which] = u0;
     const int live = min(C::kRows, s.rows - r0);
+    if ((from_before || goes_on) && lane == 0) edge[which] = {u0, u0 + s.tiles, b, kvh, r0, live};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float2 pm0 = both(A.pm[nt][0]), pm1 = both(A.pm[nt][1]);
@@ -784,7 +805,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
   __syncthreads();
 
   // ---- units that the CTA's warps share, added up row by row by warps in turn ----
-  const int e = lane < 2 * kWarps ? edge[lane] : -1;
+  const int e = lane < 2 * kWarps ? edge[lane].u0 : -1;
   const int cta0 = range[0].x0, cta1 = range[kWarps].x0;
   if (p.direct && cta0 == cta1) {  // rows that see no key
     const Seq z = load_seq<NT>(p, blockIdx.y);
@@ -799,17 +820,10 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     const int first = __ffs(todo) - 1, unit0 = __shfl_sync(0xffffffffu, e, first);
     const unsigned parts = __ballot_sync(0xffffffffu, e == unit0);
     todo &= ~parts;
-    int ub = range[first >> 1].seq, ubase = range[first >> 1].base;  // its sequence, or one before it
-    Seq us = load_seq<NT>(p, ub);
-    while (unit0 >= ubase + us.total(p.nkv)) {
-      ubase += us.total(p.nkv);
-      us = load_seq<NT>(p, ++ub);
-    }
-    const int unit = (unit0 - ubase) / us.tiles, head = unit / us.rb, row0 = (unit - head * us.rb) * C::kRows;
-    const int live = min(C::kRows, us.rows - row0);
-    const bool whole = cta0 <= unit0 && unit0 + us.tiles <= cta1;
-    const int part = 2 * blockIdx.x + (cta0 >= unit0 ? 0 : 1);
-    for (int row = 0; row < live; ++row, ++turn) {
+    const Edge u = edge[first];
+    const bool whole = cta0 <= u.u0 && u.u1 <= cta1;
+    const int part = 2 * blockIdx.x + (cta0 >= u.u0 ? 0 : 1);
+    for (int row = 0; row < u.live; ++row, ++turn) {
       if (turn % kWarps != warp) continue;
       float2 v = make_float2(-INFINITY, 0.f);
       if (parts >> lane & 1u) v = ml[lane * C::kRows + row];
@@ -826,12 +840,12 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       for (unsigned left = parts; left; left &= left - 1) {
         const int w = __ffs(left) - 1;
         const float fw = __shfl_sync(0xffffffffu, f, w);
-        const float4 u = *reinterpret_cast<const float4*>(part_row(w, row) + (lane ^ (2 * (row & 3))) * 4);
-        o = make_float4(o.x + fw * u.x, o.y + fw * u.y, o.z + fw * u.z, o.w + fw * u.w);
+        const float4 x = *reinterpret_cast<const float4*>(part_row(w, row) + (lane ^ (2 * (row & 3))) * 4);
+        o = make_float4(o.x + fw * x.x, o.y + fw * x.y, o.z + fw * x.z, o.w + fw * x.w);
       }
       if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        write_row4(p, ub, head, row0 + row, lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        write_row4(p, u.seq, u.head, u.row0 + row, lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       } else {
         *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(part) * C::kRows + row) * kHD + lane * 4) = o;
         if (lane == 0) p.part_ml[part * C::kRows + row] = make_float2(M, L);

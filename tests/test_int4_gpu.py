@@ -367,6 +367,45 @@ def test_broken_keys_reach_the_rows_that_see_them_and_no_others():
             assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("nh", [1, 2, 4])
+def test_broken_values_behind_a_row_leave_it_as_it_is(nh):
+    """Only V is broken, and 1, 2 or 4 heads of the group put rows with and without it into one warp."""
+    ops, g = _ops(), _gen(21)
+    n, P = 90, 16
+    for P in (8, 16):
+        pages, table, slots = _filled(g, [n], 1, P)
+        v = torch.full((1, 1, 128), float("nan"), dtype=BF, device="cuda")
+        ops.kv_store_int4(_randn(g, 1, 1, 128).to(BF), v, slots[0][88:89], pages)
+        q, pos = _randn(g, 1, 3, nh, 128).to(BF), torch.tensor([87], device="cuda")
+        for ctas in (0, 1):
+            out = ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=n, num_ctas=ctas)
+            assert out[0, 1:].isnan().all()
+            _check(out[:, :1], q[:, :1], pages, [slots[0][:88]], pos)
+
+
+def test_value_scales_far_apart():
+    """Groups of values 2^40 apart, tokens too: each is held to its own size."""
+    ops, g = _ops(), _gen(22)
+    n, P = 700, 16
+    pages, table, slots = _filled(g, [n], 2, P)
+    v = _randn(g, n, 2, 4, 32) * torch.tensor([1e-18, 1.0, 1e12, 30.0], device="cuda")[:, None]
+    v[300:] *= 1e3  # the powers of two are lowered half way
+    ops.kv_store_int4(_randn(g, n, 2, 128).to(BF), v.view(n, 2, 128).to(BF), slots[0], pages)
+    q, pos = _randn(g, 1, 1, 8, 128).to(BF), torch.tensor([n - 1], device="cuda")
+    for ctas in (0, 1):
+        _check(ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=n, num_ctas=ctas), q, pages, slots, pos)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 1e4, 1e25])
+def test_query_rows_of_any_size(size):
+    ops, g = _ops(), _gen(23)
+    pages, table, slots = _filled(g, [500], 2, 16)
+    q = (_randn(g, 1, 1, 8, 128) * size).to(BF)
+    q[0, 0, 3] = 0
+    pos, scale = torch.tensor([499], device="cuda"), 0.1 / size
+    _check(ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=500, scale=scale), q, pages, slots, pos, scale=scale)
+
+
 def test_a_call_gives_the_same_bits_every_time():
     ops, g = _ops(), _gen(13)
     pages, table, _ = _filled(g, [3000, 17, 800], 8, 16)
