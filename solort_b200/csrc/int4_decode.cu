@@ -94,11 +94,17 @@ struct Params {
   int2* span;       // [batch][nkv][row block] its first part, and the CTA of its last
   int rb;           // row blocks of q_len tokens
   int batch, q_len, nh, nkv, group, max_kv_len;
+  uint32_t group_mul;  // n / group = umulhi(n, group_mul) >> group_shift for 0 <= n < 2^31, group > 1
+  int group_shift;
   int direct;  // grid (head and row block, sequence): no parts
   int ctas;
   int stable_prefix;
   float scale_log2;
 };
+
+__device__ __forceinline__ int by_group(const Params& p, int n) {
+  return p.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), p.group_mul) >> p.group_shift);
+}
 
 struct Seq {  // one sequence's share of the list
   long long qpos;
@@ -362,7 +368,8 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
           const float old = e ? was.y : was.x;
           const float now = __uint_as_float(static_cast<uint32_t>(max(253 - static_cast<int>(bits >> 7), 1)) << 23);
           sf[e] = bits ? fminf(old, now) : old;
-          f[e] = sf[e] / old;
+          const int down = static_cast<int>(__float_as_uint(sf[e]) >> 23) - static_cast<int>(__float_as_uint(old) >> 23);
+          f[e] = down < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + down) << 23);  // sf / old
         }
         A.sf[q] = pair(sf[0], sf[1]);
 #pragma unroll
@@ -472,7 +479,7 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
 }
 
 __device__ __forceinline__ void write_row4(const Params& p, int b, int kvh, int r, int c, float4 v) {
-  const int i = r / p.group, h = kvh * p.group + r - i * p.group;
+  const int i = by_group(p, r), h = kvh * p.group + r - i * p.group;
   uint2 pk;
   pk.x = pack_bf16x2(v.x, v.y);
   pk.y = pack_bf16x2(v.z, v.w);
@@ -646,28 +653,41 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     }
     commit_copies();
   };
-  int issued = x0;
-  resolve(x0);
-  if (early) {  // tiles that no earlier kernel on the stream still writes
-    for (; issued < x0 + kDepth - 1 && !(moving >> (issued - x0) & 1u); ++issued) issue(issued);
-    pdl_wait();
-  }
-  for (; issued < x0 + kDepth - 1; ++issued) issue(issued);
-
-  // ---- the warp's segments: its parts of the units (sequence, head, row block) in [x0, x1) ----
-  for (int x = x0; x < x1;) {
-    Seq s = load_seq<NT>(p, b);
+  // The unit of tile x: its sequence, its place in the list, KV head and first row, the last token that
+  // every row sees, and this lane's query rows.
+  Seq s;
+  int unit = 0, u0 = 0, seg_end = 0, kvh = 0, r0 = 0, all_see = 0;
+  const bf16* rows[NT];
+  auto enter = [&](int x) {
+    s = load_seq<NT>(p, b);
     while (x >= base + s.total(p.nkv)) {
       base += s.total(p.nkv);
       s = load_seq<NT>(p, ++b);
     }
-    const int unit = (x - base) / s.tiles;
-    const int u0 = base + unit * s.tiles;  // the unit's first tile
-    const int seg_end = min(u0 + s.tiles, x1);
-    const int kvh = unit / s.rb;
-    const int r0 = (unit - kvh * s.rb) * C::kRows;
-    // Tokens past it are not seen by every row of the segment.
-    const int all_see = static_cast<int>(min(max(s.qpos + r0 / p.group, -1ll), s.kv_end - 1ll));
+    unit = (x - base) / s.tiles;
+    u0 = base + unit * s.tiles;
+    seg_end = min(u0 + s.tiles, x1);
+    kvh = unit / s.rb;
+    r0 = (unit - kvh * s.rb) * C::kRows;
+    all_see = static_cast<int>(min(max(s.qpos + by_group(p, r0), -1ll), s.kv_end - 1ll));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + nt * 4 + (g >> 1), i = by_group(p, r);
+      rows[nt] = r < s.rows ? p.q + b * p.q_sb + i * p.q_st + (kvh * p.group + r - i * p.group) * p.q_sh + 8 * t
+                            : nullptr;
+    }
+  };
+  int issued = x0;
+  resolve(x0);
+  if (early) {  // tiles that no earlier kernel on the stream still writes
+    for (; issued < x0 + kDepth - 1 && !(moving >> (issued - x0) & 1u); ++issued) issue(issued);
+  }
+  if (x0 < x1) enter(x0);
+  if (early) pdl_wait();
+  for (; issued < x0 + kDepth - 1; ++issued) issue(issued);
+
+  // ---- the warp's segments: its parts of the units (sequence, head, row block) in [x0, x1) ----
+  for (int x = x0; x < x1;) {
     uint32_t qf[NT][4][2], qm[NT][2];
     float fr[NT];
     Acc<NT> A;
@@ -675,14 +695,11 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     // bytes the dims 32 grp + 8t + {0, 2, 4, 6} and + {1, 3, 5, 7}; scores come out times 2^-9 2^e.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 4 + (g >> 1);
-      const int i = r / p.group;
-      const bf16* from = p.q + b * p.q_sb + i * p.q_st + (kvh * p.group + r - i * p.group) * p.q_sh + 8 * t;
       uint4 v[4];
       uint32_t big = 0;
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp) {
-        v[grp] = r < s.rows ? *reinterpret_cast<const uint4*>(from + 32 * grp) : make_uint4(0u, 0u, 0u, 0u);
+        v[grp] = rows[nt] ? *reinterpret_cast<const uint4*>(rows[nt] + 32 * grp) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int d = 0; d < 4; ++d) big = __vmaxu2(big, word(v[grp], d) & 0x7fff7fffu);
       }
@@ -756,7 +773,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int r = r0 + nt * 4 + t;
-          const long long last = min(s.qpos + r / p.group, static_cast<long long>(s.kv_end) - 1);
+          const long long last = min(s.qpos + by_group(p, r), static_cast<long long>(s.kv_end) - 1);
           lim[nt] = r < s.rows ? static_cast<int>(max(last, -1ll)) : -1;
         }
       }
@@ -787,7 +804,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       const bool mine = !from_before && !goes_on;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (!mine && g == 0) ml[which * C::kRows + row] = make_float2(A.off[nt], l);
-      const int i = (r0 + row) / p.group, h = kvh * p.group + r0 + row - i * p.group;
+      const int i = by_group(p, r0 + row), h = kvh * p.group + r0 + row - i * p.group;
       bf16* to = p.out + b * p.o_sb + i * p.o_st + h * p.o_sh + 4 * g;
 #pragma unroll
       for (int grp = 0; grp < 4; ++grp) {
@@ -801,6 +818,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
         }
       }
     }
+    if (x < x1) enter(x);
   }
   __syncthreads();
 
@@ -1090,6 +1108,10 @@ extern "C" int solort_attn_decode_int4(const SolortInt4DecodeArgs* a, void* stre
   p.nh = a->num_qo_heads;
   p.nkv = a->num_kv_heads;
   p.group = a->num_qo_heads / a->num_kv_heads;
+  int log = 0;  // ceil(log2(group))
+  while ((1ll << log) < p.group) ++log;
+  p.group_mul = static_cast<uint32_t>(((1ull << (31 + log)) + p.group - 1) / p.group);
+  p.group_shift = log - 1;
   p.max_kv_len = a->max_kv_len;
   p.direct = pl.direct ? 1 : 0;
   p.ctas = pl.ctas;
