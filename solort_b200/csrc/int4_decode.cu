@@ -48,7 +48,9 @@ namespace i4 {
 constexpr int kTile = 32;                     // tokens of a tile: four blocks
 constexpr int kTileBytes = 4 * kBlockBytes;   // 5120
 constexpr int kUnitCost = 2;                  // tiles' worth of set-up of a (sequence, head, row block)
-constexpr int kDirectTiles = 16;              // up to this many tiles a (sequence, head) is one CTA
+constexpr int kDirectSteps = 6;               // the most tiles a warp takes where a unit is one CTA
+constexpr int kSplitSteps = 3;                // what the division between CTAs and its merge cost, in tiles
+constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
 // A row's running maximum is raised only when a score passes it by 2^kLazy; p is 2^kPShift there, so
 // that x stays below 2^15, inside f16.
 constexpr float kLazy = 7.f;
@@ -640,7 +642,15 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
         for (int u = 0; u < 2 * kBlockBytes; u += 512)
           if (u < size) copy16(dst + u, from + u);
       };
-      if (by_block) {
+      if ((((e.x ^ 2u) | (e.z ^ 2u)) & 15u) == 0) {  // two runs of two blocks, as most tiles are
+        const char* f0 = reinterpret_cast<const char*>(static_cast<unsigned long long>(e.y) << 32 | (e.x & ~15u)) + lane * 16;
+        const char* f1 = reinterpret_cast<const char*>(static_cast<unsigned long long>(e.w) << 32 | (e.z & ~15u)) + lane * 16;
+#pragma unroll
+        for (int u = 0; u < 2 * kBlockBytes; u += 512) {
+          copy16(to + u, f0 + u);
+          copy16(to + 2 * kBlockBytes + u, f1 + u);
+        }
+      } else if (by_block) {
         const uint4 f = lds128(places + i * 32 + 16);
         copy(e.x, e.y, to);
         copy(e.z, e.w, to + kBlockBytes);
@@ -978,13 +988,18 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   int rc = current_device_info(&di);
   if (rc != SOLORT_OK) return rc;
   pl->rb = static_cast<int>(rb);
-  pl->direct = tiles - kUnitCost <= kDirectTiles && a->num_ctas == 0;
-  if (pl->direct) return SOLORT_OK;
   const int64_t most = (tiles * units * a->batch + warps - 1) / warps;
   const int64_t wave = a->num_ctas > 0 ? a->num_ctas
                                        : static_cast<int64_t>(di.sm_count) *
                                              (pl->nt == 1 ? Cfg<1>::kCtasPerSm : Cfg<2>::kCtasPerSm);
   if (wave > (1 << 20)) return SOLORT_ERR_UNSUPPORTED;
+  // A unit is one CTA where all of them are resident at once and a warp's tiles are no more than its
+  // positions of the divided list and the division's own cost.
+  const int64_t steps = (tiles - kUnitCost + warps - 1) / warps;
+  pl->direct = a->num_ctas == 0 && units * a->batch <= wave && steps <= kDirectSteps &&
+               steps <= (most + wave - 1) / wave + kSplitSteps;
+  // The workspace never shrinks as a size grows: one for the largest call serves the smaller ones.
+  if (pl->direct && tiles - kUnitCost <= kBareTiles) return SOLORT_OK;
   pl->ctas = static_cast<int>(most < wave ? most : wave);
   const size_t parts = static_cast<size_t>(2) * pl->ctas * 4 * pl->nt;
   pl->o_bytes = parts * kHD * 4;
