@@ -730,7 +730,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
           const __nv_bfloat162 lo = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w),
                                             *reinterpret_cast<const __nv_bfloat162*>(&hi));
           const uint32_t e = g & 1 ? *reinterpret_cast<const uint32_t*>(&lo) : hi;
-          two[d] = e4m3x2(lo_bf16(e) * f, hi_bf16(e) * f);
+          const float2 ef = both(mul2(pair(lo_bf16(e), hi_bf16(e)), dup(f)));
+          two[d] = e4m3x2(ef.x, ef.y);
         }
         const uint32_t w0 = __byte_perm(two[0], two[1], 0x5410), w1 = __byte_perm(two[2], two[3], 0x5410);
         const uint32_t k[2] = {__byte_perm(w0, w1, 0x6420), __byte_perm(w0, w1, 0x7531)};
@@ -853,23 +854,26 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     const int part = 2 * blockIdx.x + (cta0 >= u.u0 ? 0 : 1);
     for (int row = 0; row < u.live; ++row, ++turn) {
       if (turn % kWarps != warp) continue;
-      float2 v = make_float2(-INFINITY, 0.f);
-      if (parts >> lane & 1u) v = ml[lane * C::kRows + row];
-      float M = v.y == 0.f ? -INFINITY : v.x;  // a part that sees no key of the row does not count
+      float2 v[kWarps];
+      float4 x[kWarps];
 #pragma unroll
-      for (int o = 1; o <= 8; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      const float f = v.y == 0.f ? 0.f : ex2(v.x - M);
-      float L = f * v.y;
-#pragma unroll
-      for (int o = 1; o <= 8; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-      M = __shfl_sync(0xffffffffu, M, 0);
-      L = __shfl_sync(0xffffffffu, L, 0);
+      for (int w = 0; w < kWarps; ++w) {  // a warp has one part of a unit at most, as its first or its last
+        const unsigned has = parts >> (2 * w) & 3u;
+        const int at = 2 * w + static_cast<int>(has >> 1);
+        v[w] = has ? ml[at * C::kRows + row] : make_float2(-INFINITY, 0.f);
+        x[w] = has ? *reinterpret_cast<const float4*>(part_row(at, row) + (lane ^ (2 * (row & 3))) * 4)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float M = -INFINITY, L = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (unsigned left = parts; left; left &= left - 1) {
-        const int w = __ffs(left) - 1;
-        const float fw = __shfl_sync(0xffffffffu, f, w);
-        const float4 x = *reinterpret_cast<const float4*>(part_row(w, row) + (lane ^ (2 * (row & 3))) * 4);
-        o = make_float4(o.x + fw * x.x, o.y + fw * x.y, o.z + fw * x.z, o.w + fw * x.w);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        if (v[w].y != 0.f) M = fmaxf(M, v[w].x);  // a part that sees no key of the row does not count
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = v[w].y == 0.f ? 0.f : ex2(v[w].x - M);
+        L += f * v[w].y;
+        o = make_float4(o.x + f * x[w].x, o.y + f * x[w].y, o.z + f * x[w].z, o.w + f * x[w].w);
       }
       if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
