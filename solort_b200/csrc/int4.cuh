@@ -109,29 +109,32 @@ __device__ __forceinline__ f2 quotient2(f2 a, f2 minus_b, f2 y) {
 // (lo, hi: with NaN going on) reads back as NaN throughout: a broken input stays visible.
 //
 // The quotients by the step are quotient2's, its reciprocal from the hardware's approximation and one
-// Newton step (correctly rounded for every bf16 step); a step outside 2^+-90 takes true divisions. No
-// code needs clamping: step >= need (1 - 2^-23), so that d / step lies within 7.5 (1 + 2^-22) and its
-// sum with 7.5 rounds to 0..15.
+// Newton step (correctly rounded for every bf16 step). Where the step is far from 1 values, mid and step
+// are scaled by 2^+-64 first, which changes no quotient: mid is then below 2^-60, or what underflows is
+// lost in the sum with 7.5 in any case. No code needs clamping: step >= need (1 - 2^-23), so that
+// d / step lies within 7.5 (1 + 2^-22) and its sum with 7.5 rounds to 0..15.
 struct Quantiser {
-  f2 m2, s2, y2;
-  float step;
+  f2 f, m2, s2, y2;
   uint32_t meta;
-  bool plain;
 
   __device__ __forceinline__ Quantiser(float lo, float hi) {
     const float mid = __bfloat162float(
         __float2bfloat16_rn(__fadd_rn(__fmul_rn(0.5f, lo), __fmul_rn(0.5f, hi))));
     const float wide = max_nan(__fsub_rn(hi, mid), __fsub_rn(mid, lo));
-    plain = wide >= 0x1p-86f && wide <= 0x1p90f;
     constexpr float kSeventh = 1.f / 7.5f;
     const float n0 = __fmul_rn(wide, kSeventh);
     float need = fmaf(fmaf(-n0, 7.5f, wide), kSeventh, n0);
-    if (__builtin_expect(!plain, 0)) need = __fdiv_rn(wide, 7.5f);
+    float by = 1.f;
+    if (__builtin_expect(!(wide >= 0x1p-86f && wide <= 0x1p90f), 0)) {
+      need = __fdiv_rn(wide, 7.5f);
+      by = wide == 0.f ? 1.f : wide < 1.f ? 0x1p64f : 0x1p-64f;
+    }
     const uint32_t sbits = (__float_as_uint(need) + 0xffffu) & 0xffff0000u;  // need >= 0
-    step = sbits ? __uint_as_float(sbits) : 1.f;
+    const float step = (sbits ? __uint_as_float(sbits) : 1.f) * by;
     float y0;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(step));
-    m2 = dup(-mid);
+    f = dup(by);
+    m2 = dup(-mid * by);
     s2 = dup(-step);
     y2 = dup(fmaf(fmaf(-step, y0, 1.f), y0, y0));
     meta = wide < INFINITY ? __byte_perm(sbits, __float_as_uint(mid), 0x7632) : 0x7fff7fffu;
@@ -142,14 +145,7 @@ struct Quantiser {
     uint32_t w = 0;
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      const f2 d = add2(x[i], m2);
-      f2 q;
-      if (__builtin_expect(plain, 1)) {
-        q = quotient2(d, s2, y2);
-      } else {
-        const float2 v = both(d);
-        q = pair(__fdiv_rn(v.x, step), __fdiv_rn(v.y, step));
-      }
+      const f2 q = quotient2(fma2(x[i], f, m2), s2, y2);
       const float2 r = both(add2(add2(q, dup(7.5f)), dup(12582912.f)));
       w = (w << 4) + __float_as_uint(r.y);
       w = (w << 4) + __float_as_uint(r.x);
