@@ -237,17 +237,22 @@ __device__ __forceinline__ void store_group(uint8_t* blk, int i, int g, bool is_
   reinterpret_cast<uint32_t*>(blk + (is_value ? kOffVScale : kOffKScale) + 16 * i)[g] = meta;
 }
 
-// The values of eight codes as bf16: mid + scale (code - 7.5), whose product is exact in fp32. A code
-// one bit up in the low bits of 2^22 is the float 2^22 + code.
+// The values of eight codes as bf16: mid + scale (code - 7.5), whose product is exact in fp32. Nibble n of
+// a word in the low bits of 2^23 is the float 2^23 + 16^n code, and the scale takes 16^-n.
 __device__ __forceinline__ uint4 held8(uint32_t codes, uint32_t meta) {
-  const f2 s = dup(lo_bf16(meta)), mid = dup(hi_bf16(meta)), centre = dup(-4194311.5f);
+  const f2 s = dup(lo_bf16(meta)), mid = dup(hi_bf16(meta));
+  const f2 s12 = mul2(s, pair(0x1p-4f, 0x1p-8f)), s34 = mul2(s, pair(0x1p-12f, 0x1p-16f));
+  const f2 centre12 = pair(-0x1p23f - 7.5f * 16, -0x1p23f - 7.5f * 256);
+  const f2 centre34 = pair(-0x1p23f - 7.5f * 4096, -0x1p23f - 7.5f * 65536);
   uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t a = i ? codes >> (8 * i - 1) : codes << 1, b = codes >> (8 * i + 3);
-    const f2 c = add2(pair(__uint_as_float(a & 0x1eu | 0x4a800000u), __uint_as_float(b & 0x1eu | 0x4a800000u)), centre);
-    const float2 v = both(fma2(s, c, mid));
-    o[i] = pack_bf16x2(v.x, v.y);
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t w = h ? codes >> 12 : codes << 4;  // the half's codes are nibbles 1 to 4
+    auto at = [&](uint32_t nibble) { return __uint_as_float(w & nibble | 0x4b000000u); };
+    const float2 a = both(fma2(s12, add2(pair(at(0xf0u), at(0xf00u)), centre12), mid));
+    const float2 b = both(fma2(s34, add2(pair(at(0xf000u), at(0xf0000u)), centre34), mid));
+    o[2 * h] = pack_bf16x2(a.x, a.y);
+    o[2 * h + 1] = pack_bf16x2(b.x, b.y);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }

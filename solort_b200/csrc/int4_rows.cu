@@ -215,12 +215,12 @@ __global__ void __launch_bounds__(kRowThreads) store_kernel(const StoreParams p)
   pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x & 3;
-  const bool is_v = static_cast<int>(blockIdx.y) >= p.nkv;  // K heads, then V heads
-  const int head = blockIdx.y - (is_v ? p.nkv : 0);
+  const bool is_v = static_cast<int>(blockIdx.x) >= p.nkv;  // K heads, then V heads
+  const int head = blockIdx.x - (is_v ? p.nkv : 0);
   const bf16* src = (is_v ? p.value + head * p.v_sh : p.key + head * p.k_sh) + g * 32;
   const int64_t st = is_v ? p.v_st : p.k_st;
-  const int step = gridDim.x * kGroupRowsPerCta;
-  int tok = blockIdx.x * kGroupRowsPerCta + (threadIdx.x >> 2);
+  const int step = gridDim.y * kGroupRowsPerCta;
+  int tok = blockIdx.y * kGroupRowsPerCta + (threadIdx.x >> 2);
   uint4 u[4];
   if (tok < p.t)
 #pragma unroll
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kRowThreads) load_kernel(const LoadParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int l8 = threadIdx.x & 7, t = l8 & 3, g = l8 >> 2;
-  const int head = blockIdx.y;
-  const int tok = blockIdx.x * kRowsPerCta + (threadIdx.x >> 3);
+  const int head = blockIdx.x;
+  const int tok = (blockIdx.z * gridDim.y + blockIdx.y) * kRowsPerCta + (threadIdx.x >> 3);
   if (tok >= p.t) return;
   const long long slot = p.slots[tok];
   if (!row_there(slot, p.ar, l8 == 0)) return;
@@ -301,10 +301,10 @@ int make_arena(const void* pages, int64_t page_stride, int64_t head_stride, int3
 }
 
 template <typename P>
-int launch_rows(void (*kernel)(const P), const P& prm, int64_t x, int64_t y, void* stream) {
+int launch_rows(void (*kernel)(const P), const P& prm, int64_t x, int64_t y, int64_t z, void* stream) {
   if (x > (1ll << 30) || y > 65535) return SOLORT_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y), static_cast<unsigned>(z));
   cfg.blockDim = dim3(kRowThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute at[1];
@@ -382,7 +382,7 @@ extern "C" int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* 
   p.heads = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
   p.q_ctas = (a->num_qo_heads + p.heads - 1) / p.heads;
   p.kv_ctas = (a->num_kv_heads + p.heads - 1) / p.heads;
-  return i4::launch_rows(i4::append_kernel, p, x, p.q_ctas + 2ll * p.kv_ctas, stream);
+  return i4::launch_rows(i4::append_kernel, p, x, p.q_ctas + 2ll * p.kv_ctas, 1, stream);
 }
 
 extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* stream) {
@@ -410,8 +410,8 @@ extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* str
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
   const int64_t y = 2ll * a->num_kv_heads;
-  return i4::launch_rows(i4::store_kernel, p, i4::token_ctas(a->num_tokens, i4::kGroupRowsPerCta, y, di), y,
-                         stream);
+  return i4::launch_rows(i4::store_kernel, p, y, i4::token_ctas(a->num_tokens, i4::kGroupRowsPerCta, y, di),
+                         1, stream);
 }
 
 extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* stream) {
@@ -438,6 +438,6 @@ extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* strea
   p.t = a->num_tokens;
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
-  return i4::launch_rows(i4::load_kernel, p, (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta,
-                         a->num_kv_heads, stream);
+  const int64_t all = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta, wide = 32768;
+  return i4::launch_rows(i4::load_kernel, p, a->num_kv_heads, all < wide ? all : wide, (all + wide - 1) / wide, stream);
 }
