@@ -7,7 +7,7 @@
 // The scale is rounded up and measured from the rounded mid, so no value falls off the ends of the
 // code range, however far the group lies from zero. Codes are symmetric about 7.5: a product with
 // (code - 7.5) stays as small as the values themselves, which is what bounds the error that the
-// attention's bf16 probabilities add.
+// attention's rounded probabilities add.
 //
 // Layout: pages of P tokens (a power of two >= 8), one KV head of a page contiguous, P / 8 blocks
 // of 8 tokens of kBlockBytes. Every byte belongs to one token, so rows are written without a

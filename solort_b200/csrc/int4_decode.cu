@@ -4,32 +4,42 @@
 //   q . k       = sum_g scale_g sum_d q_d c_d + (mid_g - 7.5 scale_g) sum_d q_d
 //   sum_t p v_d = sum_t (p scale_g) c_d + sum_t p (mid_g - 7.5 scale_g)
 // so the tensor cores multiply the codes themselves and the scales are applied to their fp32 results
-// (keys) or to the probabilities (values): the cache is never expanded. The products run in e4m3,
-// because a nibble in a byte IS an e4m3 number: bytes 0..15 are the subnormals and the first binade,
-// the values c 2^-9 exactly. Eight codes become operands with a shift and two ands, half of what a
-// bf16 operand costs, and the e4m3 product takes a quarter of the bf16 one's time per multiply-add
-// (measured: m16n8k32 e4m3 4.6 cycles a scheduler, m16n8k16 bf16 8.8; results exact to fp32).
+// (keys) or to the probabilities (values): the cache is never expanded.
 //
-// The other operand is split in two e4m3 numbers, hi and lo, four significant bits each, lo times
-// 16; they are the two columns of one query row. A query row is scaled by a power of two to a
+// Keys: a nibble in a byte IS an e4m3 number. Bytes 0..15 are the subnormals and the first binade, the
+// values c 2^-9 exactly, so eight codes become operands with a shift and two ands, and an e4m3 product
+// takes a quarter of a bf16 one's time per multiply-add (measured: m16n8k32 e4m3 4.6 cycles a scheduler,
+// m16n8k16 bf16 8.8). The query is split in two e4m3 numbers, hi and lo, four significant bits each, lo
+// times 16; they are the two columns of one query row. A query row is scaled by a power of two to a
 // maximum in [128, 256): hi + lo / 16 is then its bf16 values exactly down to 2^-13 of the row's maximum,
-// and within 2^-22 of that maximum below. For values it is x = 2^8 p scale sf, with p relative to the
-// row's running maximum and sf the power of two that brings the group's scales below 1: hi + lo / 16 is
-// within 2^-9 x (2^-8 next to a power of two: bf16's half step), and again within 2^-22 of the maximum
-// for x below 2^-13 of it. The codes are centred with the sum of the same numbers (a product with
-// ones), O = sum x c - 7.5 sum x + sum p mid, so that their rounding weighs |v - mid| and not c.
+// and within 2^-22 of that maximum below. The mids' and -7.5 scales' share is one bf16 product more, of
+// the held scales and mids with the query's group sums (themselves split in two bf16 numbers).
 //
-// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k32, tokens or dims as the 16
-// rows), so that four query rows fill an n8 tile; P^T turns into the second product's operand with
-// movmatrix, two tokens' bytes to an element.
+// Values: a nibble in a half is an f16 subnormal, c 2^-24 or 16 c 2^-24, which costs a shift and ands
+// too and lets the other operand keep 11 bits: x = 2^8 p scale sf, with p relative to the row's running
+// maximum (at most 2^7 until that is raised) and sf the power of two that brings the group's scales
+// below 1. x is within 2^-11 of itself, and within 2^-25 below 2^-14. The codes are centred with the
+// sum of the same numbers (a product with ones), O = sum x c - 7.5 sum x + sum p mid, so that their
+// rounding weighs |v - mid| and not c. p, its sum, sum p mid and all accumulators are fp32.
 //
-// Work split: the cache's 32-token tiles, over all sequences, KV heads and blocks of query rows, are
-// one list, and CTA c of n takes the tiles [T c / n, T (c + 1) / n): sequences of any lengths load
-// every SM alike, and the workspace is two partials per CTA whatever the batch. A CTA's eight warps
-// take its tiles in turn, each warp with a ring of kDepth tiles of its own (5120 bytes a tile, one bulk
-// copy for each page that it touches, an mbarrier), so warps meet only at the end of a (sequence, head)
-// segment. A segment that is a whole (sequence, head) writes its final rows; parts meet in
-// merge_kernel. Lengths are read on the device, and merge_kernel repeats the same division.
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (tokens or dims as the 16 rows), so that
+// four query rows fill an n8 tile of the first and a row pair a column pair of the second; P^T turns into
+// its operand with movmatrix.
+//
+// Work split: the cache's 32-token tiles, over all sequences, KV heads and blocks of query rows, are one
+// list, divided evenly over all warps of the GPU, so that sequences of any lengths load every SM alike. A
+// unit (a sequence's KV head and row block) counts kUnitCost tiles more for its set-up: 48 sequences of
+// 127 to 8111 keys take 34.9 us with 2, 34.3 with 4, 35.2 with 8. A warp has a ring of kDepth tiles of its
+// own (5120 bytes a tile, in 16-byte asynchronous copies), so warps meet only when a unit that they share
+// ends. A unit that lies within a CTA is added up there; parts of several CTAs meet in merge_kernel,
+// through `span`. Lengths are read on the device. Short caches skip the division: a unit is a CTA
+// (make_plan).
+//
+// Bound by memory for up to four rows: 32 query heads over 8 KV heads, 131072 keys 38.3 us (4.4 TB/s; 5.8
+// TB/s for each key beyond 16384, of 6.57 measured for a copy). The rest is what every call pays, 7.2 us
+// at 1000 keys: the way of the query rows into operands, a first tile that nothing hides, the sums of
+// the parts and the merge's launch. Blocks of eight rows are bound by the instructions of a tile, 771 a
+// warp, 60 of them matrix products: 8 sequences of 5 rows, 4099 keys 26.3 us.
 //
 // Reference semantics: src/solort/model/cuda_graph_executor.py:168,180-184 (keys 0..pos), :250
 // (query i at vpos0 + i), src/solort/cache/kv_cache.py:136-149 (slot = bt[pos // P] * P + pos % P).
@@ -47,7 +57,7 @@ namespace i4 {
 
 constexpr int kTile = 32;                     // tokens of a tile: four blocks
 constexpr int kTileBytes = 4 * kBlockBytes;   // 5120
-constexpr int kUnitCost = 2;                  // tiles' worth of set-up of a (sequence, head, row block)
+constexpr int kUnitCost = 4;                  // tiles' worth of set-up of a unit
 constexpr int kDirectSteps = 6;               // the most tiles a warp takes where a unit is one CTA
 constexpr int kSplitSteps = 3;                // what the division between CTAs and its merge cost, in tiles
 constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
@@ -58,14 +68,16 @@ constexpr float kPShift = 15.f - kLazy;
 constexpr float kCodeUnit = 512.f;         // a key code's e4m3 value is c / 512
 constexpr float kValueUnit = 16777216.f;   // a value code's f16 value is c 2^-24, or 16 c 2^-24
 
-// NT n8 tiles of four query rows each. One: 160 registers a thread and 111 KB, so that two CTAs of six
-// warps share an SM. Two: one CTA of eight warps with all the registers that they can have.
+// NT n8 tiles of four query rows each; two CTAs of six warps share an SM, 168 registers a thread. A third
+// tile in the ring, which fits for four rows, gains nothing (131072 keys 39.0 us, 38.3 without). For eight
+// rows (8 sequences of 5 rows, 4099 keys 26.5 us) eight warps of 255 registers are as fast; ten warps load
+// the four schedulers unevenly (30.3 us); sixteen rows a block want 255 registers and spill (32.9 us).
 template <int NT>
 struct Cfg {
   static constexpr int kWarps = 6;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kCtasPerSm = 2;
-  static constexpr int kDepth = NT == 1 ? 3 : 2;  // tiles of a warp in shared memory
+  static constexpr int kDepth = 2;  // tiles of a warp in shared memory
   static constexpr int kRows = 4 * NT;
   static constexpr int kRing = kWarps * kDepth * kTileBytes;
   static constexpr int kRed = kWarps * kRows * kHD * 4;
@@ -267,7 +279,8 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
     {
       // sum_g (mid_g - 7.5 scale_g) sum_d q_d, a product itself: k = mids, mids, scales, scales of the four
       // groups against the sums of q, their low parts, and both times -7.5.
-      const uint2 n0 = lds64(b0 + kOffKScale + 16 * g + 8 * (t & 1)), n1 = lds64(b1 + kOffKScale + 16 * g + 8 * (t & 1));
+      const uint32_t at = kOffKScale + 16 * g + 8 * (t & 1);
+      const uint2 n0 = lds64(b0 + at), n1 = lds64(b1 + at);
       const uint32_t a[4] = {__byte_perm(n0.x, n0.y, 0x7632), __byte_perm(n1.x, n1.y, 0x7632),
                              __byte_perm(n0.x, n0.y, 0x5410), __byte_perm(n1.x, n1.y, 0x5410)};
 #pragma unroll
@@ -370,7 +383,8 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
           const float old = e ? was.y : was.x;
           const float now = __uint_as_float(static_cast<uint32_t>(max(253 - static_cast<int>(bits >> 7), 1)) << 23);
           sf[e] = bits ? fminf(old, now) : old;
-          const int down = static_cast<int>(__float_as_uint(sf[e]) >> 23) - static_cast<int>(__float_as_uint(old) >> 23);
+          const int down = static_cast<int>(__float_as_uint(sf[e]) >> 23) -
+                           static_cast<int>(__float_as_uint(old) >> 23);
           f[e] = down < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + down) << 23);  // sf / old
         }
         A.sf[q] = pair(sf[0], sf[1]);
@@ -635,16 +649,18 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
         const unsigned blocks = by_block ? b0 | b1 << 1 | b2 << 2 | b3 << 3 : b0 * 3u | b1 * 12u;
         gone = (gone & ~(15u << (4 * slot))) | blocks << (4 * slot);
       }
+      auto source = [&](uint32_t lo, uint32_t hi) {
+        return reinterpret_cast<const char*>(static_cast<unsigned long long>(hi) << 32 | (lo & ~15u)) + lane * 16;
+      };
       auto copy = [&](uint32_t lo, uint32_t hi, uint32_t dst) {
-        const char* from = reinterpret_cast<const char*>(static_cast<unsigned long long>(hi) << 32 | (lo & ~15u)) + lane * 16;
+        const char* from = source(lo, hi);
         const int size = static_cast<int>(lo & 3u) * kBlockBytes - lane * 16;
 #pragma unroll
         for (int u = 0; u < 2 * kBlockBytes; u += 512)
           if (u < size) copy16(dst + u, from + u);
       };
       if ((((e.x ^ 2u) | (e.z ^ 2u)) & 15u) == 0) {  // two runs of two blocks, as most tiles are
-        const char* f0 = reinterpret_cast<const char*>(static_cast<unsigned long long>(e.y) << 32 | (e.x & ~15u)) + lane * 16;
-        const char* f1 = reinterpret_cast<const char*>(static_cast<unsigned long long>(e.w) << 32 | (e.z & ~15u)) + lane * 16;
+        const char *f0 = source(e.x, e.y), *f1 = source(e.z, e.w);
 #pragma unroll
         for (int u = 0; u < 2 * kBlockBytes; u += 512) {
           copy16(to + u, f0 + u);
@@ -756,7 +772,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       }
       qm[nt][0] = g & 1 ? 0u : pack_bf16x2(z0, z1);
       qm[nt][1] = g & 1 ? 0u : pack_bf16x2(y0, y1);
-      fr[nt] = p.scale_log2 * kCodeUnit * __uint_as_float(static_cast<uint32_t>(127 - __shfl_sync(0xffffffffu, up, 8 * t)) << 23);
+      const int row_up = __shfl_sync(0xffffffffu, up, 8 * t);
+      fr[nt] = p.scale_log2 * kCodeUnit * __uint_as_float(static_cast<uint32_t>(127 - row_up) << 23);
       A.l[nt] = 0.f, A.off[nt] = 0.f, A.top[nt] = -INFINITY;
       A.pm[nt][0] = A.pm[nt][1] = 0;
     }
@@ -976,7 +993,8 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
     return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->num_qo_heads % a->num_kv_heads != 0) return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->batch > 65535) return SOLORT_ERR_UNSUPPORTED;
-  // One n8 tile, four rows, where they fit it (two CTAs per SM), else blocks of eight rows.
+  // Four rows a block where they fit one, else eight: a tile of eight takes 1.25 of four's time (1217 and
+  // 977 cycles a scheduler), which two blocks of four would take twice.
   const int64_t rows = static_cast<int64_t>(a->q_len) * (a->num_qo_heads / a->num_kv_heads);
   pl->nt = rows <= 4 ? 1 : 2;
   const int warps = pl->nt == 1 ? Cfg<1>::kWarps : Cfg<2>::kWarps;
@@ -998,7 +1016,9 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
                                              (pl->nt == 1 ? Cfg<1>::kCtasPerSm : Cfg<2>::kCtasPerSm);
   if (wave > (1 << 20)) return SOLORT_ERR_UNSUPPORTED;
   // A unit is one CTA where all of them are resident at once and a warp's tiles are no more than its
-  // positions of the divided list and the division's own cost.
+  // positions of the divided list and the division's own cost. 32 heads over 8, one CTA a unit against
+  // the division: 1 x 512 keys 7.2 and 7.4 us, 1 x 1024 10.2 and 8.2, 16 x 768 10.8 and 12.6, 16 x 1536
+  // 17.0 and 15.1; 64 x 8 units of 5-row sequences do not fit at once, 256 keys: 40.9 and 31.2.
   const int64_t steps = (tiles - kUnitCost + warps - 1) / warps;
   pl->direct = a->num_ctas == 0 && units * a->batch <= wave && steps <= kDirectSteps &&
                steps <= (most + wave - 1) / wave + kSplitSteps;
@@ -1046,7 +1066,8 @@ int launch(const Params& prm, const Plan& pl, void* stream) {
   if (cudaLaunchKernelEx(&cfg, decode_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   int rc = launch_status();
   if (rc != SOLORT_OK || pl.direct) return rc;
-  // Few rows have many parts each, and want many warps; of many rows most have one, and want to leave.
+  // Few rows have many parts each and want many warps (131072 keys, 32 rows: 8 warps 38.9 us, 2 warps
+  // 41.4); of many rows most are written already and want to leave (48 sequences, 1536 rows: 39.2 and 35.4).
   const int rows = prm.batch * prm.q_len * prm.nh;
   cfg = pdl_config(dim3(rows), (rows <= pl.ctas ? kMergeWarps : 2) * 32, 0, stream, attr);
   if (cudaLaunchKernelEx(&cfg, merge_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;

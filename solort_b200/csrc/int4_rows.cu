@@ -14,9 +14,10 @@
 // exchanged. A CTA works on tokens of one head, which share the cache lines that they write; the
 // append's query CTAs go over several heads, with the tokens' RoPE rows in registers.
 //
-// All three are bound by the bytes they move, and for a decode step by their launch. 8 KV heads:
-// storing 16380 rows MEASURE_STORE, loading 32001 rows MEASURE_LOAD; appending a prompt of 8190
-// tokens with 32 query heads MEASURE_APPEND.
+// All three are bound by the bytes they move, and for a decode step by their launch. 8 KV heads: storing
+// 16380 rows 17.6 us (5.0 TB/s), loading 32001 rows 30.8 us (5.6 TB/s), appending a prompt of 8190 tokens
+// with 32 query heads 38.1 us (4.8 TB/s: a token's RoPE rows wait for its position, and 96 registers
+// leave 20 warps an SM to hide that); one token's append 2.2 us.
 #include <math.h>
 
 #include "host_util.h"
@@ -31,7 +32,9 @@ namespace i4 {
 constexpr int kRowThreads = 128;
 constexpr int kRowsPerCta = kRowThreads / 8;
 constexpr int kGroupRowsPerCta = kRowThreads / 4;  // of four lanes a row
-constexpr int kFullCtas = 16;  // CTAs per SM from which a CTA takes more than one round of rows
+// CTAs per SM from which a CTA takes more than one round of rows, or heads: 16380 rows stored 18.8 us with
+// 8, 17.6 with 16, 18.1 with 32; a prompt of 8190 tokens appended 38.1 us with 16, 41.7 with 32.
+constexpr int kFullCtas = 16;
 
 struct Arena {
   uint8_t* base;
@@ -376,9 +379,11 @@ extern "C" int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* 
   p.q_out = static_cast<bf16*>(a->q_out);
   p.qo_st = a->q_out_stride_token;
   p.qo_sh = a->q_out_stride_head;
-  // One head per CTA while the GPU is not full, and up to eight.
+  // One head per CTA while the GPU is not full, and up to eight (prompt of 8190 tokens: at most four 41.7
+  // us, eight 38.1).
   const int64_t x = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta;
-  const int64_t per = x * (a->num_qo_heads + 2ll * a->num_kv_heads) / (static_cast<int64_t>(di.sm_count) * i4::kFullCtas);
+  const int64_t full = static_cast<int64_t>(di.sm_count) * i4::kFullCtas;
+  const int64_t per = x * (a->num_qo_heads + 2ll * a->num_kv_heads) / full;
   p.heads = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
   p.q_ctas = (a->num_qo_heads + p.heads - 1) / p.heads;
   p.kv_ctas = (a->num_kv_heads + p.heads - 1) / p.heads;
@@ -438,6 +443,8 @@ extern "C" int solort_attn_kv_load_int4(const SolortInt4LoadArgs* a, void* strea
   p.t = a->num_tokens;
   p.nkv = a->num_kv_heads;
   p.slots = a->slots;
-  const int64_t all = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta, wide = 32768;
-  return i4::launch_rows(i4::load_kernel, p, a->num_kv_heads, all < wide ? all : wide, (all + wide - 1) / wide, stream);
+  const int64_t wide = 32768;
+  const int64_t all = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta;
+  return i4::launch_rows(i4::load_kernel, p, a->num_kv_heads, all < wide ? all : wide,
+                         (all + wide - 1) / wide, stream);
 }
