@@ -487,13 +487,15 @@ SOLORT_API int solort_attn_kv_load_int4(const SolortInt4LoadArgs* args, void* st
 /*
  * GQA attention of q_len query tokens per sequence over the 4-bit pages: solort_attn_decode with a
  * block table (q, out, q_pos, q_lens, max_kv_len, block_table and the SOLORT_DECODE_STABLE_PREFIX
- * flag as there), for any q_len: the rows of a KV head are taken in blocks of 16. Rows that see no
- * key are zero; rows past q_lens are not written. Keys behind a block-table entry outside the arena
+ * flag as there), for any q_len: the rows of a KV head are taken in blocks of 8 (4 where there are no
+ * more). Rows that see no key are zero; rows past q_lens are not written. Keys behind a block-table entry outside the arena
  * count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
  * elements; out 8-byte aligned, multiples of 4. The workspace (256-byte aligned; query its size with
- * the same args) depends on the device and the row count, not on the lengths or the batch past one
- * wave of CTAs; calls that share one must be ordered on their streams. num_ctas: 0 = one resident
- * wave, otherwise the number of CTAs over which the keys are divided.
+ * the same args) is 0 for short caches, else two partial results a CTA of one resident wave and 8 bytes
+ * per sequence, KV head and row block; it never shrinks as batch, q_len or max_kv_len grow, so one for
+ * the largest call serves the smaller ones. Nothing in it outlives a call; calls that share one must be
+ * ordered on their streams. num_ctas: 0 = one resident wave, otherwise the number of CTAs over which
+ * the keys are divided.
  */
 typedef struct SolortInt4DecodeArgs {
   const void* q;

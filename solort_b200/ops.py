@@ -626,7 +626,8 @@ def qk_norm_rope_append_int4(
 def decode_int4_workspace_bytes(batch: int, q_len: int, num_qo_heads: int, num_kv_heads: int,
                                 max_kv_len: int, *, num_ctas: int = 0) -> int:
     """Workspace bytes a :func:`gqa_decode_paged_int4` call with these sizes needs on the current
-    device (0 up to 256 keys; some MiB at most, whatever the batch and the lengths)."""
+    device: 0 for short caches, else some MiB and 8 bytes per sequence, KV head and block of 8 rows. It
+    never shrinks as a size grows, so a workspace of the largest call serves the smaller ones."""
     return _calls_int4.decode_workspace_bytes(batch, q_len, num_qo_heads, num_kv_heads, max_kv_len,
                                               num_ctas)
 
@@ -660,8 +661,11 @@ def gqa_decode_paged_int4(
     if workspace is None:
         _, a = _calls_int4.decode_args(q, kv_pages, block_table, q_pos, out, int(max_kv_len), scale,
                                        q_lens, int(num_ctas), stable_prefix)
-        need = _calls_int4.decode_workspace_bytes(a.batch, a.q_len, a.num_qo_heads, a.num_kv_heads,
-                                                  a.max_kv_len, a.num_ctas) if q.numel() else 0
+        need = 0
+        if q.numel():
+            with torch.cuda.device(q.device):
+                need = _calls_int4.decode_workspace_bytes(a.batch, a.q_len, a.num_qo_heads,
+                                                          a.num_kv_heads, a.max_kv_len, a.num_ctas)
         workspace = (torch.empty(need, dtype=torch.uint8, device=q.device) if need
                      else _empty_workspace(q.device))
     (_calls_int4.decode_into if _plain(kv_pages) else _OPS.gqa_decode_paged_int4)(

@@ -5,12 +5,13 @@
 * Load returns the held values rounded to bf16 exactly (``mid + scale * (code - 7.5)`` has one fp32
   rounding before the bf16 one).
 * Attention, per element, against the 64-bit sum over the held values: half a bf16 step of the result,
-  2^-8 |o|; half a bf16 step of each p * scale, in all at most 2^-8 sum p |v - mid|; and the fp32 parts. Of
-  these a score's error enters p relatively: a score is a sum of four groups, each of products up to
-  143 |q| scale whose fp32 accumulation loses at most 2^-20 of the largest partial sum over its 32
-  terms, scaled by 128^-0.5: below 2^-9 * 2^-3 for |q| scale <= 8 -- the inputs here stay below -- and
-  the accumulation of p scale * code loses 2^-24 of partial sums below 143 / 7.5 times sum p |v - mid|'s
-  bound per 16-token step. Both are covered by 2^-10 sum p |v|.
+  2^-8 |o|; half an f16 step of each p * scale, in all at most 2^-11 sum p |v - mid| (below 2^-14 of the
+  tile's largest the step is 2^-25 of that, 2^-33 of the row's, which a thousand keys do not add up to
+  2^-22); and the fp32 parts. Of these a score's error enters p relatively: a score is a sum of four
+  groups, each of products up to 143 |q| scale whose fp32 accumulation loses at most 2^-20 of the largest
+  partial sum over its 32 terms, scaled by 128^-0.5: below 2^-9 * 2^-3 for |q| scale <= 8 -- the inputs
+  here stay below -- and the accumulation of p scale * code loses 2^-24 of partial sums below 143 / 7.5
+  times sum p |v - mid|'s bound per 16-token step. Both are covered by 2^-10 sum p |v|.
 """
 
 from __future__ import annotations
@@ -75,7 +76,7 @@ def _check(out, q, pages, slots, q_pos, scale=128 ** -0.5, q_lens=None, kept=Non
         k, v, m = Q.load(pages, sl, mids=True)
         ref, near, size = Q.attention(q[b, :t], k, v, int(q_pos[b]), scale, m)
         off = (out[b, :t].double() - ref).abs()
-        tol = 2.0 ** -8 * (ref.abs() + near) + 2.0 ** -10 * size + 1e-30
+        tol = 2.0 ** -8 * ref.abs() + 2.0 ** -11 * near + 2.0 ** -10 * size + 1e-30
         assert torch.isfinite(out[b, :t]).all(), f"sequence {b}"
         worst = (off / tol).max().item() if off.numel() else 0.0
         assert worst <= 1, f"sequence {b} of {len(sl)} keys: {worst:.3g} of the tolerance"
@@ -130,6 +131,29 @@ def test_exact_halves_between_two_codes_round_as_the_oracles():
     ref, slots = pages.clone(), torch.arange(200, device="cuda")
     ops.kv_store_int4(v, -v, slots, pages)
     Q.store(ref, slots, v, -v)
+    assert torch.equal(pages, ref)
+
+
+def test_rows_of_every_magnitude_give_the_oracles_bytes():
+    """Steps from the least subnormal to the greatest bf16 number, groups of one value and of two. A mid of
+    zero counts without its sign: of +0 and -0 either is the least (IEEE 754), and both hold the same value
+    (here the oracle's own bytes differ between devices)."""
+    ops, g = _ops(), _gen(24)
+    x = torch.rand(272, 1, 128, generator=g, device="cuda", dtype=torch.float64) * 2 - 1
+    x = (x * 2.0 ** torch.arange(-143, 129, device="cuda", dtype=torch.float64)[:, None, None])
+    x = x.clamp(-3.3895e38, 3.3895e38).to(BF)
+    x[:, 0, 32:64] = x[:, 0, 32:33]
+    x[:, 0, 64:96] = torch.where(torch.arange(32, device="cuda") % 3 == 0, x[:, 0, 64:65], x[:, 0, 65:66])
+    y = x.roll(1, 2)  # a group takes one value of its neighbour's
+    pages = ops.kv_pages_int4(34, 1, 8)
+    ref, slots = pages.clone(), torch.arange(272, device="cuda")
+    ops.kv_store_int4(x, y, slots, pages)
+    Q.store(ref, slots, x, y)
+    for block in (pages, ref):
+        words = block.view(34, 1280).view(torch.int16)
+        for at in (256, 576):  # scales and mids of the keys, of the values
+            mids = words[:, at + 1:at + 64:2]
+            mids.masked_fill_(mids == -0x8000, 0)
     assert torch.equal(pages, ref)
 
 
@@ -413,6 +437,80 @@ def test_a_call_gives_the_same_bits_every_time():
     first = ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=3000)
     for _ in range(5):
         assert torch.equal(ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=3000), first)
+
+
+@pytest.mark.parametrize("batch,nkv,n", [(16, 8, 1152), (16, 8, 1153), (37, 8, 192), (38, 8, 192),
+                                         (150, 8, 33), (3, 1, 513)])
+def test_both_sides_of_the_division_between_ctas(batch, nkv, n):
+    _run([n - 7 * (b % 4) for b in range(batch)], 2 * nkv, nkv, 16, max_kv_len=n)
+
+
+def test_a_workspace_of_the_largest_call_serves_the_smaller_ones():
+    ops, g = _ops(), _gen(25)
+    sizes = [[ops.decode_int4_workspace_bytes(b, t, 32, 8, n) for n in (1, 64, 512, 513, 1100, 4000, 70000)]
+             for t in (1, 2, 3, 9) for b in (1, 2, 4, 16, 38, 64, 300)]
+    by = torch.tensor(sizes).view(4, 7, 7)
+    for dim in range(3):
+        assert (by.diff(dim=dim) >= 0).all()
+    pages, table, slots = _filled(g, [1100] * 4, 8, 16)
+    ws = torch.full((ops.decode_int4_workspace_bytes(4, 5, 32, 8, 1100),), 255, dtype=U8, device="cuda")
+    for b, t, n in ((4, 5, 1100), (1, 1, 700), (2, 2, 1), (4, 1, 1100), (3, 5, 300), (1, 5, 1000)):
+        q = _randn(g, b, t, 32, 128).to(BF)
+        pos = torch.full((b,), n - 1, device="cuda")
+        out = ops.gqa_decode_paged_int4(q, pages, table[:b], pos, max_kv_len=n, workspace=ws)
+        _check(out, q, pages, [x[:n] for x in slots[:b]], pos)
+
+
+def test_calls_on_two_streams_at_once():
+    ops, g = _ops(), _gen(26)
+    pages, table, _ = _filled(g, [5000, 900, 2111], 8, 16)
+    q = [_randn(g, 3, t, 32, 128).to(BF) for t in (1, 4)]
+    pos = torch.tensor([4990, 890, 2101], device="cuda")
+    want = [ops.gqa_decode_paged_int4(x, pages, table, pos, max_kv_len=5000) for x in q]
+    ws = [torch.empty(ops.decode_int4_workspace_bytes(3, x.shape[1], 32, 8, 5000), dtype=U8, device="cuda")
+          for x in q]
+    out = [torch.zeros_like(x) for x in q]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, w, o, st in zip(q, ws, out, streams):
+            with torch.cuda.stream(st):
+                ops.gqa_decode_paged_int4(x, pages, table, pos, max_kv_len=5000, out=o, workspace=w)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_two_graphs_that_share_a_workspace_and_sequences_that_share_pages():
+    """Two captured calls of different sizes, replayed in turn over one workspace; the second's sequences
+    are one prefix at several lengths, the same pages in every table row."""
+    ops, g = _ops(), _gen(27)
+    pages, table, slots = _filled(g, [3000], 8, 16)
+    shared = table.expand(5, -1).contiguous()
+    ends = [2999, 2999, 40, 1500, 0]
+    q = [_randn(g, b, 1, 32, 128).to(BF) for b in (1, 5)]
+    pos = [torch.tensor([2000], device="cuda"), torch.tensor(ends, device="cuda")]
+    ws = torch.empty(ops.decode_int4_workspace_bytes(5, 1, 32, 8, 3000), dtype=U8, device="cuda")
+    out = [torch.zeros_like(x) for x in q]
+
+    def call(i):
+        ops.gqa_decode_paged_int4(q[i], pages, (table, shared)[i], pos[i], max_kv_len=3000, out=out[i], workspace=ws)
+
+    graphs = []
+    for i in range(2):
+        call(i)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            call(i)
+    for _ in range(3):
+        for x in out:
+            x.fill_(9)
+        pos[0] += 1
+        for gr in graphs + graphs[::-1]:
+            gr.replay()
+        torch.cuda.synchronize()
+        _check(out[0], q[0], pages, slots, pos[0])
+        _check(out[1], q[1], pages, slots * 5, pos[1])
 
 
 def test_refusals_on_the_device():
