@@ -7,6 +7,7 @@ writes only the tensors it is given and allocates nothing. Errors raise ``Runtim
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -54,23 +55,48 @@ def _rows(name: str, t: torch.Tensor, n: int, heads: int) -> None:
           f"{name} must be bf16 [{n}, {heads}, {HEAD_DIM}] with a contiguous head dim")
 
 
-def _launch(name: str, args, index: int) -> None:
-    fn = _FN.get(name)
-    if fn is None:
-        fn = _FN[name] = getattr(_lib.load(), name)
-    if index == _current_device():
-        rc = fn(_byref(args), _stream_at(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(_byref(args), _stream_at(index))
-    if rc:
-        _lib.check(rc, name)
-
-
-_FN: dict[str, object] = {}
 # torch's raw getter: what torch.cuda.current_device() returns, less its look at the lazy start (the
 # tensors of a call are on the device already).
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_CODE = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint32: "I",
+         ctypes.c_float: "f", ctypes.c_size_t: "N"}
+_PROTOTYPE = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
+
+
+def packer(args: type[ctypes.Structure]):
+    """``pack(*fields)``: the bytes of a struct of that type with these fields, in a third of the time
+    that building the struct takes."""
+    layout = "@" + "".join(_CODE[t] for _, t in args._fields_)
+    return struct.Struct(f"{layout}{ctypes.sizeof(args) - struct.calcsize(layout)}x").pack
+
+
+def _entry(name: str, args: type[ctypes.Structure]):
+    """``call(index, *fields)``: the library's ``name`` on the current stream of device ``index``."""
+    pack, fn = packer(args), None
+
+    def call(index: int, *fields) -> None:
+        nonlocal fn
+        if fn is None:
+            fn = _PROTOTYPE((name, _lib.load()))
+        try:
+            packed = pack(*fields)
+        except struct.error as e:
+            raise RuntimeError(f"{name}: {e}") from None
+        if index == _current_device():
+            rc = fn(packed, _stream_at(index))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(packed, _stream_at(index))
+        if rc:
+            _lib.check(rc, name)
+
+    return call
+
+
+_append = _entry("solort_attn_qk_norm_rope_append_int4", _lib.SolortInt4AppendArgs)
+_store = _entry("solort_attn_kv_store_int4", _lib.SolortInt4StoreArgs)
+_load = _entry("solort_attn_kv_load_int4", _lib.SolortInt4LoadArgs)
+_decode = _entry("solort_attn_decode_int4", _lib.SolortInt4DecodeArgs)
 
 
 # The conditions of a call are looked at together first, since a decode step's calls are as short as
@@ -83,7 +109,7 @@ def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positio
     t = qkv.shape[0]
     pages, cs, outs = kv_pages.shape, cos.shape, q_out.shape
     index = qkv.get_device()
-    sp, so, sc = kv_pages.stride(), q_out.stride(), cos.stride()
+    sp, so, sc, sx = kv_pages.stride(), q_out.stride(), cos.stride(), qkv.stride()
     P = pages[-1] // TOKEN_BYTES
     if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
             P * TOKEN_BYTES == pages[2] and len(outs) == 3 and len(cs) == 2 and index >= 0 and
@@ -93,12 +119,12 @@ def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positio
             _BF16 is qkv.dtype is q_out.dtype is cos.dtype is sin.dtype is q_norm_weight.dtype is
             k_norm_weight.dtype and _I64 is positions.dtype is slots.dtype and
             outs == (t, outs[1], HEAD_DIM) and so[2] == 1 and
-            qkv.shape == (t, (outs[1] + 2 * pages[1]) * HEAD_DIM) and qkv.stride(1) == 1 and
+            qkv.shape == (t, (outs[1] + 2 * pages[1]) * HEAD_DIM) and sx[1] == 1 and
             q_norm_weight.shape == k_norm_weight.shape == (HEAD_DIM,) and
-            q_norm_weight.stride(0) == 1 == k_norm_weight.stride(0) and
+            q_norm_weight.is_contiguous() and k_norm_weight.is_contiguous() and
             cs == sin.shape and cs[1] == HEAD_DIM and sc == sin.stride() and sc[1] == 1 and
-            positions.shape == slots.shape == (t,) and
-            (t < 2 or positions.stride(0) == 1 == slots.stride(0))):
+            positions.shape == slots.shape == (t,) and positions.is_contiguous() and
+            slots.is_contiguous()):
         page_size(kv_pages)
         _same_device(qkv, ("kv_pages", kv_pages), ("q_out", q_out), ("cos", cos), ("sin", sin),
                      ("positions", positions), ("slots", slots),
@@ -115,14 +141,13 @@ def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positio
         _vector("slots", slots, _I64, t)
         raise RuntimeError("cos and sin must be bf16 [rows, 128] tables with equal strides and "
                            "contiguous rows")
-    _launch("solort_attn_qk_norm_rope_append_int4", _lib.SolortInt4AppendArgs(
-        qkv.data_ptr(), qkv.stride(0), t, outs[1], pages[1], HEAD_DIM, q_norm_weight.data_ptr(),
-        k_norm_weight.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), sc[0], cs[0],
-        positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), so[0], so[1],
-        kv_pages.data_ptr(), sp[0], sp[1], P, pages[0]), index)
+    _append(index, qkv.data_ptr(), sx[0], t, outs[1], pages[1], HEAD_DIM, q_norm_weight.data_ptr(),
+            k_norm_weight.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), sc[0], cs[0],
+            positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), so[0], so[1],
+            kv_pages.data_ptr(), sp[0], sp[1], P, pages[0])
 
 
-def _key_value(what, key, value, slots, kv_pages):
+def _key_value(call, key, value, slots, kv_pages) -> None:
     pages, sp = kv_pages.shape, kv_pages.stride()
     sk, sv, index, n = key.stride(), value.stride(), key.get_device(), slots.numel()
     P = pages[-1] // TOKEN_BYTES
@@ -130,33 +155,31 @@ def _key_value(what, key, value, slots, kv_pages):
             P * TOKEN_BYTES == pages[2] and index >= 0 and
             index == value.get_device() == slots.get_device() == kv_pages.get_device() and
             _BF16 is key.dtype is value.dtype and slots.dtype is _I64 and slots.shape == (n,) and
-            (n < 2 or slots.stride(0) == 1) and
+            slots.is_contiguous() and
             key.shape == value.shape == (n, pages[1], HEAD_DIM) and sk[2] == 1 == sv[2]):
         page_size(kv_pages)
         _same_device(kv_pages, ("key", key), ("value", value), ("slots", slots))
         _vector("slots", slots, _I64, n)
         _rows("key", key, n, pages[1])
         _rows("value", value, n, pages[1])
-    return index, what(key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], n, pages[1],
-                       HEAD_DIM, slots.data_ptr(), kv_pages.data_ptr(), sp[0], sp[1], P, pages[0])
+    call(index, key.data_ptr(), value.data_ptr(), sk[0], sk[1], sv[0], sv[1], n, pages[1], HEAD_DIM,
+         slots.data_ptr(), kv_pages.data_ptr(), sp[0], sp[1], P, pages[0])
 
 
 def store_into(key, value, slots, kv_pages) -> None:
     """Quantise ``key / value [tokens, nkv, 128]`` to ``slots``: ``solort_attn::kv_store_int4``."""
-    index, args = _key_value(_lib.SolortInt4StoreArgs, key, value, slots, kv_pages)
-    _launch("solort_attn_kv_store_int4", args, index)
+    _key_value(_store, key, value, slots, kv_pages)
 
 
 def load_into(kv_pages, slots, key, value) -> None:
     """The held values at ``slots`` to ``key / value``: ``solort_attn::kv_load_int4``."""
-    index, args = _key_value(_lib.SolortInt4LoadArgs, key, value, slots, kv_pages)
-    _launch("solort_attn_kv_load_int4", args, index)
+    _key_value(_load, key, value, slots, kv_pages)
 
 
-def decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: float | None, q_lens,
-                num_ctas: int, stable_prefix: bool):
-    """Checked and packed arguments of a decode call without its workspace, and the device index."""
-    shape, pages, table = q.shape, kv_pages.shape, block_table.shape
+def decode_fields(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: float | None, q_lens,
+                  num_ctas: int) -> tuple:
+    """The device index and the checked fields of a decode call before its workspace."""
+    shape, pages, table, st = q.shape, kv_pages.shape, block_table.shape, block_table.stride()
     sq, so, sp, index = q.stride(), out.stride(), kv_pages.stride(), q.get_device()
     P = pages[-1] // TOKEN_BYTES
     if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
@@ -164,9 +187,8 @@ def decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: fl
             index == kv_pages.get_device() == block_table.get_device() == q_pos.get_device() ==
             out.get_device() and _BF16 is q.dtype is out.dtype and block_table.dtype is _I32 and
             q_pos.dtype is _I64 and shape[3] == HEAD_DIM and sq[3] == 1 and out.shape == shape and
-            so[3] == 1 and table[0] == shape[0] and (table[1] < 2 or block_table.stride(1) == 1) and
-            0 < max_kv_len <= table[1] * P and q_pos.shape == shape[:1] and
-            (shape[0] < 2 or q_pos.stride(0) == 1)):
+            so[3] == 1 and table[0] == shape[0] and (table[1] < 2 or st[1] == 1) and
+            0 < max_kv_len <= table[1] * P and q_pos.shape == shape[:1] and q_pos.is_contiguous()):
         page_size(kv_pages)
         _same_device(q, ("kv_pages", kv_pages), ("block_table", block_table), ("q_pos", q_pos),
                      ("out", out))
@@ -175,7 +197,7 @@ def decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: fl
         _need(out.dtype is _BF16 and out.shape == shape and so[3] == 1,
               "out must be bf16, of the shape of q, with a contiguous head dim")
         _need(block_table.dtype is _I32 and len(table) == 2 and table[0] == shape[0] and
-              (table[1] < 2 or block_table.stride(1) == 1),
+              (table[1] < 2 or st[1] == 1),
               "block_table must be int32 [batch, max_pages] with contiguous rows")
         _need(0 < max_kv_len <= table[1] * P,
               f"max_kv_len must be in 1..{table[1] * P}, the keys a block-table row can hold, "
@@ -184,12 +206,10 @@ def decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: fl
     if q_lens is not None:
         _need(q_lens.device == q.device, f"q_lens is on {q_lens.device}, not on {q.device}")
         _vector("q_lens", q_lens, _I32, shape[0])
-    return index, _lib.SolortInt4DecodeArgs(
-        q.data_ptr(), sq[0], sq[1], sq[2], out.data_ptr(), so[0], so[1], so[2], kv_pages.data_ptr(),
-        sp[0], sp[1], P, pages[0], block_table.data_ptr(), block_table.stride(0), q_pos.data_ptr(),
-        None if q_lens is None else q_lens.data_ptr(), shape[0], shape[1], shape[2], pages[1],
-        HEAD_DIM, max_kv_len, _SCALE if scale is None else scale, num_ctas, None, 0,
-        _lib.DECODE_STABLE_PREFIX if stable_prefix else 0)
+    return (index, q.data_ptr(), sq[0], sq[1], sq[2], out.data_ptr(), so[0], so[1], so[2],
+            kv_pages.data_ptr(), sp[0], sp[1], P, pages[0], block_table.data_ptr(), st[0], q_pos.data_ptr(),
+            0 if q_lens is None else q_lens.data_ptr(), shape[0], shape[1], shape[2], pages[1], HEAD_DIM,
+            max_kv_len, _SCALE if scale is None else scale, num_ctas)
 
 
 _SCALE = HEAD_DIM ** -0.5
@@ -200,15 +220,14 @@ def decode_into(q, kv_pages, block_table, q_pos, out, workspace, max_kv_len: int
                 stable_prefix: bool = False) -> None:
     """``out = attention(q, 4-bit pages)``: the body of ``solort_attn::gqa_decode_paged_int4``. A short
     or misaligned workspace is the library's SOLORT_ERR_WORKSPACE, raised as ``RuntimeError``."""
-    index, a = decode_args(q, kv_pages, block_table, q_pos, out, max_kv_len, scale, q_lens, num_ctas,
-                           stable_prefix)
-    n = workspace.numel()
-    if n:
-        _need(workspace.get_device() == index, f"workspace is on {workspace.device}, not on {q.device}")
+    fields = decode_fields(q, kv_pages, block_table, q_pos, out, max_kv_len, scale, q_lens, num_ctas)
+    at = n = 0
+    if workspace.numel():
+        _need(workspace.get_device() == fields[0], f"workspace is on {workspace.device}, not on {q.device}")
         _need(workspace.is_contiguous(), "workspace must be contiguous")
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), n * workspace.element_size()
+        at, n = workspace.data_ptr(), workspace.nbytes
     if q.numel():
-        _launch("solort_attn_decode_int4", a, index)
+        _decode(*fields, at, n, _lib.DECODE_STABLE_PREFIX if stable_prefix else 0)
 
 
 def decode_workspace_bytes(batch: int, q_len: int, num_qo_heads: int, num_kv_heads: int,

@@ -659,13 +659,13 @@ def gqa_decode_paged_int4(
     if out is None:
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     if workspace is None:
-        _, a = _calls_int4.decode_args(q, kv_pages, block_table, q_pos, out, int(max_kv_len), scale,
-                                       q_lens, int(num_ctas), stable_prefix)
+        _calls_int4.decode_fields(q, kv_pages, block_table, q_pos, out, int(max_kv_len), scale, q_lens,
+                                  int(num_ctas))
         need = 0
         if q.numel():
             with torch.cuda.device(q.device):
-                need = _calls_int4.decode_workspace_bytes(a.batch, a.q_len, a.num_qo_heads,
-                                                          a.num_kv_heads, a.max_kv_len, a.num_ctas)
+                need = _calls_int4.decode_workspace_bytes(*q.shape[:3], kv_pages.shape[1], int(max_kv_len),
+                                                          int(num_ctas))
         workspace = (torch.empty(need, dtype=torch.uint8, device=q.device) if need
                      else _empty_workspace(q.device))
     (_calls_int4.decode_into if _plain(kv_pages) else _OPS.gqa_decode_paged_int4)(

@@ -10,7 +10,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from oracle import int4 as Q
-from solort_b200 import _lib, ops, torch_ops_int4
+from solort_b200 import _calls_int4, _lib, ops, torch_ops_int4
 from tests.test_capi import _c_layout
 
 BF, I32, I64, U8 = torch.bfloat16, torch.int32, torch.int64, torch.uint8
@@ -82,6 +82,14 @@ def test_ctypes_struct_matches_header(name):
     assert c["sizeof"] == ctypes.sizeof(cls)
     for f, _ in cls._fields_:
         assert c[f] == getattr(cls, f).offset, f
+
+
+@pytest.mark.parametrize("name", ["SolortInt4AppendArgs", "SolortInt4StoreArgs", "SolortInt4LoadArgs",
+                                  "SolortInt4DecodeArgs"])
+def test_packed_fields_are_the_struct(name):
+    cls = getattr(_lib, name)
+    fields = [0.25 * i if t is ctypes.c_float else (1 << 30) + i for i, (_, t) in enumerate(cls._fields_)]
+    assert _calls_int4.packer(cls)(*fields) == bytes(cls(*fields))
 
 
 def test_ops_are_registered_with_their_outputs_mutated():

@@ -532,6 +532,9 @@ def test_refusals_on_the_device():
                                      pos, pos, pages, num_qo_heads=32, num_kv_heads=4)
     with pytest.raises(RuntimeError, match="cpu"):
         ops.gqa_decode_paged_int4(q, pages, table.cpu(), pos, max_kv_len=600)
+    with pytest.raises(RuntimeError, match="solort_attn_decode_int4"):  # a count beyond its field
+        ops.gqa_decode_paged_int4(q, pages, table, pos, max_kv_len=600, num_ctas=1 << 40,
+                                  workspace=torch.empty(need, dtype=U8, device="cuda"))
 
 
 # ---------------------------------------------------------------------------------------------
