@@ -32,14 +32,14 @@
 // 127 to 8111 keys take 34.9 us with 2, 34.3 with 4, 35.2 with 8. A warp has a ring of kDepth tiles of its
 // own (5120 bytes a tile, in 16-byte asynchronous copies), so warps meet only when a unit that they share
 // ends. A unit that lies within a CTA is added up there; parts of several CTAs meet in merge_kernel,
-// through `span`. Lengths are read on the device. Short caches skip the division: a unit is a CTA
-// (make_plan).
+// through `span`. Lengths are read on the device. Short caches skip the division: a unit is a CTA, or a
+// cluster of CTAs that add up their sums over shared memory (make_plan).
 //
 // Bound by memory for up to four rows: 32 query heads over 8 KV heads, 131072 keys 38.3 us (4.4 TB/s; 5.8
-// TB/s for each key beyond 16384, of 6.57 measured for a copy). The rest is what every call pays, 7.2 us
-// at 1000 keys: the way of the query rows into operands, a first tile that nothing hides, the sums of
-// the parts and the merge's launch. Blocks of eight rows are bound by the instructions of a tile, 771 a
-// warp, 60 of them matrix products: 8 sequences of 5 rows, 4099 keys 26.3 us.
+// TB/s for each key beyond 16384, of 6.57 measured for a copy). The rest is what every call pays, 6.8 us
+// at 1000 keys: the way of the query rows into operands, a first tile that nothing hides, the sums of the
+// parts and the cluster's barriers, or the merge's launch. Blocks of eight rows are bound by the
+// instructions of a tile, 771 a warp, 60 of them matrix products: 8 sequences of 5 rows, 4099 keys 26.3 us.
 //
 // Reference semantics: src/solort/model/cuda_graph_executor.py:168,180-184 (keys 0..pos), :250
 // (query i at vpos0 + i), src/solort/cache/kv_cache.py:136-149 (slot = bt[pos // P] * P + pos % P).
@@ -58,8 +58,9 @@ namespace i4 {
 constexpr int kTile = 32;                     // tokens of a tile: four blocks
 constexpr int kTileBytes = 4 * kBlockBytes;   // 5120
 constexpr int kUnitCost = 4;                  // tiles' worth of set-up of a unit
-constexpr int kDirectSteps = 6;               // the most tiles a warp takes where a unit is one CTA
-constexpr int kSplitSteps = 3;                // what the division between CTAs and its merge cost, in tiles
+constexpr int kDirectSteps = 6;               // the most tiles a warp takes where the list is not divided
+constexpr int kSplitSteps = 2;                // what the division and its merge cost more, in tiles
+constexpr int kMostCluster = 8;               // CTAs of a cluster, the portable limit
 constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
 // A row's running maximum is raised only when a score passes it by 2^kLazy; p is 2^kPShift there, so
 // that x stays below 2^15, inside f16.
@@ -87,7 +88,9 @@ struct Cfg {
   static constexpr int kOffEdge = kOffMl + 2 * kWarps * kRows * 8;
   static constexpr int kOffRange = kOffEdge + 2 * kWarps * 24;
   static constexpr int kOffPlaces = (kOffRange + (kWarps + 1) * 12 + 15) / 16 * 16;  // [warp][32 tiles][4]
-  static constexpr int kSmem = kOffPlaces + kWarps * 32 * 32;
+  static constexpr int kOffUnit = kOffPlaces + kWarps * 32 * 32;  // a CTA's sums for its cluster: [row][128]
+  static constexpr int kOffUnitMl = kOffUnit + kRows * kHD * 4;   // and [row]
+  static constexpr int kSmem = kOffUnitMl + kRows * 8;
 };
 static_assert(Cfg<1>::kSmem <= 115712, "two CTAs per SM");
 
@@ -110,7 +113,8 @@ struct Params {
   int batch, q_len, nh, nkv, group, max_kv_len;
   uint32_t group_mul;  // n / group = umulhi(n, group_mul) >> group_shift for 0 <= n < 2^31, group > 1
   int group_shift;
-  int direct;  // grid (head and row block, sequence): no parts
+  int direct;   // grid (head and row block, sequence): no parts
+  int cluster;  // then the CTAs of a unit, a cluster
   int ctas;
   int stable_prefix;
   float scale_log2;
@@ -187,6 +191,27 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Shared memory of the cluster's CTA `rank`, at this CTA's address `addr`.
+__device__ __forceinline__ uint32_t in_cluster(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 cluster_lds128(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 cluster_lds64(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
@@ -549,6 +574,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
 
   pdl_launch_dependents();
   if (lane == 0) edge[2 * warp].u0 = edge[2 * warp + 1].u0 = -1;
+  float2* unit_ml = reinterpret_cast<float2*>(smem + C::kOffUnitMl);
+  if (tid < C::kRows) unit_ml[tid] = make_float2(-INFINITY, 0.f);
   const bool early = p.stable_prefix != 0;
   if (!early) pdl_wait();
   if (warp == 0) {
@@ -556,8 +583,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     if (p.direct) {
       const Seq s = load_seq<NT>(p, blockIdx.y);
       r.seq = blockIdx.y;
-      const int unit = blockIdx.x;
-      if (unit < s.units(p.nkv)) r.x0 = unit * s.tiles + s.tiles * min(lane, kWarps) / kWarps;
+      const int unit = blockIdx.x / p.cluster, at = (blockIdx.x - unit * p.cluster) * kWarps + min(lane, kWarps);
+      if (unit < s.units(p.nkv)) r.x0 = unit * s.tiles + s.tiles * at / (p.cluster * kWarps);
     } else {
       Prefix f;
       for (int c = 0; c < p.batch; c += 32) load_prefix<NT>(p, f, c);
@@ -817,7 +844,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     }
     const int which = 2 * warp + (from_before ? 0 : 1);
     const int live = min(C::kRows, s.rows - r0);
-    if ((from_before || goes_on) && lane == 0) edge[which] = {u0, u0 + s.tiles, b, kvh, r0, live};
+    const bool mine = !from_before && !goes_on && p.cluster == 1;
+    if (!mine && lane == 0) edge[which] = {u0, u0 + s.tiles, b, kvh, r0, live};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float2 pm0 = both(A.pm[nt][0]), pm1 = both(A.pm[nt][1]);
@@ -829,7 +857,6 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
         for (int grp = 0; grp < 4; ++grp) pm[grp] += __shfl_xor_sync(0xffffffffu, pm[grp], o);
       }
       const int row = nt * 4 + t;
-      const bool mine = !from_before && !goes_on;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (!mine && g == 0) ml[which * C::kRows + row] = make_float2(A.off[nt], l);
       const int i = by_group(p, r0 + row), h = kvh * p.group + r0 + row - i * p.group;
@@ -853,7 +880,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
   // ---- units that the CTA's warps share, added up row by row by warps in turn ----
   const int e = lane < 2 * kWarps ? edge[lane].u0 : -1;
   const int cta0 = range[0].x0, cta1 = range[kWarps].x0;
-  if (p.direct && cta0 == cta1) {  // rows that see no key
+  if (p.direct && p.cluster == 1 && cta0 == cta1) {  // rows that see no key
     const Seq z = load_seq<NT>(p, blockIdx.y);
     if (static_cast<int>(blockIdx.x) >= z.units(p.nkv)) return;
     const int head = blockIdx.x / z.rb, row0 = (blockIdx.x - head * z.rb) * C::kRows;
@@ -867,7 +894,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
     const unsigned parts = __ballot_sync(0xffffffffu, e == unit0);
     todo &= ~parts;
     const Edge u = edge[first];
-    const bool whole = cta0 <= u.u0 && u.u1 <= cta1;
+    const bool whole = cta0 <= u.u0 && u.u1 <= cta1 && p.cluster == 1;
     const int part = 2 * blockIdx.x + (cta0 >= u.u0 ? 0 : 1);
     for (int row = 0; row < u.live; ++row, ++turn) {
       if (turn % kWarps != warp) continue;
@@ -895,12 +922,53 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
         write_row4(p, u.seq, u.head, u.row0 + row, lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      } else if (p.cluster > 1) {
+        *reinterpret_cast<float4*>(smem + C::kOffUnit + (row * kHD + lane * 4) * 4) = o;
+        if (lane == 0) unit_ml[row] = make_float2(M, L);
       } else {
         *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(part) * C::kRows + row) * kHD + lane * 4) = o;
         if (lane == 0) p.part_ml[part * C::kRows + row] = make_float2(M, L);
       }
     }
   }
+  if (p.cluster == 1) return;
+
+  // ---- the cluster's unit, its rows added up by the CTAs and their warps in turn ----
+  cluster_sync();
+  const Seq z = load_seq<NT>(p, blockIdx.y);
+  const int cu = blockIdx.x / p.cluster, rank = blockIdx.x - cu * p.cluster;
+  if (cu < z.units(p.nkv)) {
+    const int head = cu / z.rb, row0 = (cu - head * z.rb) * C::kRows;
+    for (int row = rank + warp * p.cluster; row < min(C::kRows, z.rows - row0); row += kWarps * p.cluster) {
+      const uint32_t at = smem_u32(smem) + C::kOffUnit + (row * kHD + lane * 4) * 4;
+      const uint32_t at_ml = smem_u32(smem) + C::kOffUnitMl + row * 8;
+      float2 v[kMostCluster];
+      float4 x[kMostCluster];
+#pragma unroll
+      for (int c = 0; c < kMostCluster; ++c) {
+        v[c] = make_float2(-INFINITY, 0.f);
+        x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < p.cluster) {
+          v[c] = cluster_lds64(in_cluster(at_ml, c));
+          if (v[c].y != 0.f) x[c] = cluster_lds128(in_cluster(at, c));
+        }
+      }
+      float M = -INFINITY, L = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < kMostCluster; ++c)
+        if (v[c].y != 0.f) M = fmaxf(M, v[c].x);
+#pragma unroll
+      for (int c = 0; c < kMostCluster; ++c) {
+        const float f = v[c].y == 0.f ? 0.f : ex2(v[c].x - M);
+        L += f * v[c].y;
+        o = make_float4(o.x + f * x[c].x, o.y + f * x[c].y, o.z + f * x[c].z, o.w + f * x[c].w);
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      write_row4(p, blockIdx.y, head, row0 + row, lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+  }
+  cluster_sync();  // no CTA leaves while its sums are read
 }
 
 // The rows whose tiles were divided between CTAs: one CTA per output row, whose warps take the parts
@@ -980,7 +1048,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
 }
 
 struct Plan {
-  int nt = 1, ctas = 1, rb = 1;
+  int nt = 1, ctas = 1, rb = 1, cluster = 1;
   bool direct = false;
   size_t o_bytes = 0, ml_bytes = 0, ws_bytes = 0;
 };
@@ -1015,15 +1083,27 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
                                        : static_cast<int64_t>(di.sm_count) *
                                              (pl->nt == 1 ? Cfg<1>::kCtasPerSm : Cfg<2>::kCtasPerSm);
   if (wave > (1 << 20)) return SOLORT_ERR_UNSUPPORTED;
-  // A unit is one CTA where all of them are resident at once and a warp's tiles are no more than its
-  // positions of the divided list and the division's own cost. 32 heads over 8, one CTA a unit against
-  // the division: 1 x 512 keys 7.2 and 7.4 us, 1 x 1024 10.2 and 8.2, 16 x 768 10.8 and 12.6, 16 x 1536
-  // 17.0 and 15.1; 64 x 8 units of 5-row sequences do not fit at once, 256 keys: 40.9 and 31.2.
-  const int64_t steps = (tiles - kUnitCost + warps - 1) / warps;
-  pl->direct = a->num_ctas == 0 && units * a->batch <= wave && steps <= kDirectSteps &&
-               steps <= (most + wave - 1) / wave + kSplitSteps;
+  // Short caches are not divided: a unit is a cluster of k CTAs with 6 k warps, where all clusters are
+  // resident at once, a warp's tiles are few, and no more than its share of the divided list and what the
+  // division costs. k is what a warp's tiles and the cluster cost least with, in quarters of a tile; two
+  // CTAs on an SM cost one more. 32 heads over 8, us with clusters of 1, 2, 4, 8 | divided:
+  //   1 x 256 keys   5.5  6.1  6.0  6.8 | 7.8      8 x 1024   11.1 10.0  9.8    - | 11.1
+  //   1 x 768        8.4  7.6  6.4  7.1 | 8.2      8 x 4096    33  22.1 16.0    - | 17.4
+  //   1 x 1536      12.8  9.8  7.9  7.2 | 7.8     16 x 1024   13.1 11.3    -    - | 12.9
+  //   1 x 4096      28   17.5 12.0  9.8 | 8.8     64 x 256    15.2    -    -    - | 15.9
+  constexpr int kClusterCost[] = {0, 4, 5, 8};
+  int64_t least = 0, steps = 0;
+  for (int i = 0; (1 << i) <= kMostCluster && (units * a->batch << i) <= wave; ++i) {
+    const int64_t of = (tiles - kUnitCost + (warps << i) - 1) / (warps << i);
+    const int64_t cost = 4 * of + kClusterCost[i] + (i && (units * a->batch << i) > di.sm_count ? 4 : 0);
+    if (i == 0 || cost < least) least = cost, steps = of, pl->cluster = 1 << i;
+  }
+  const bool bare = tiles - kUnitCost <= kBareTiles;
+  pl->direct = a->num_ctas == 0 && units * a->batch <= wave &&
+               (bare || (steps <= kDirectSteps && (steps - kSplitSteps) * wave <= most));
+  if (!pl->direct) pl->cluster = 1;
   // The workspace never shrinks as a size grows: one for the largest call serves the smaller ones.
-  if (pl->direct && tiles - kUnitCost <= kBareTiles) return SOLORT_OK;
+  if (pl->direct && bare) return SOLORT_OK;
   pl->ctas = static_cast<int>(most < wave ? most : wave);
   const size_t parts = static_cast<size_t>(2) * pl->ctas * 4 * pl->nt;
   pl->o_bytes = parts * kHD * 4;
@@ -1033,7 +1113,7 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
 }
 
 inline cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, void* stream,
-                                     cudaLaunchAttribute* attr) {
+                                     int cluster, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -1041,8 +1121,11 @@ inline cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, void* 
   cfg.stream = static_cast<cudaStream_t>(stream);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cfg;
 }
 
@@ -1060,16 +1143,16 @@ int launch(const Params& prm, const Plan& pl, void* stream) {
       return SOLORT_ERR_CUDA;
     if (dev < 32) configured.fetch_or(1u << dev, std::memory_order_release);
   }
-  cudaLaunchAttribute attr[1];
-  const dim3 grid = pl.direct ? dim3(prm.nkv * pl.rb, prm.batch) : dim3(pl.ctas);
-  cudaLaunchConfig_t cfg = pdl_config(grid, C::kThreads, C::kSmem, stream, attr);
+  cudaLaunchAttribute attr[2];
+  const dim3 grid = pl.direct ? dim3(prm.nkv * pl.rb * pl.cluster, prm.batch) : dim3(pl.ctas);
+  cudaLaunchConfig_t cfg = pdl_config(grid, C::kThreads, C::kSmem, stream, pl.cluster, attr);
   if (cudaLaunchKernelEx(&cfg, decode_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   int rc = launch_status();
   if (rc != SOLORT_OK || pl.direct) return rc;
   // Few rows have many parts each and want many warps (131072 keys, 32 rows: 8 warps 38.9 us, 2 warps
   // 41.4); of many rows most are written already and want to leave (48 sequences, 1536 rows: 39.2 and 35.4).
   const int rows = prm.batch * prm.q_len * prm.nh;
-  cfg = pdl_config(dim3(rows), (rows <= pl.ctas ? kMergeWarps : 2) * 32, 0, stream, attr);
+  cfg = pdl_config(dim3(rows), (rows <= pl.ctas ? kMergeWarps : 2) * 32, 0, stream, 1, attr);
   if (cudaLaunchKernelEx(&cfg, merge_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   return launch_status();
 }
@@ -1154,6 +1237,7 @@ extern "C" int solort_attn_decode_int4(const SolortInt4DecodeArgs* a, void* stre
   p.group_shift = log - 1;
   p.max_kv_len = a->max_kv_len;
   p.direct = pl.direct ? 1 : 0;
+  p.cluster = pl.cluster;
   p.ctas = pl.ctas;
   p.rb = pl.rb;
   p.stable_prefix = (a->flags & SOLORT_DECODE_STABLE_PREFIX) ? 1 : 0;

@@ -445,6 +445,14 @@ def test_both_sides_of_the_division_between_ctas(batch, nkv, n):
     _run([n - 7 * (b % 4) for b in range(batch)], 2 * nkv, nkv, 16, max_kv_len=n)
 
 
+@pytest.mark.parametrize("lengths,most,q_len,q_lens", [
+    ([700], 700, 1, None), ([0, 700], 700, 1, None), ([1, 1536], 1536, 1, None), ([1536, 33], 1536, 2, [2, 1]),
+    ([700, 5, 0, 64], 700, 5, [5, 3, 0, 1]), ([1] * 9 + [1000] * 7, 1000, 1, None), ([190, 3000], 3000, 3, [3, 0])])
+def test_units_of_several_ctas(lengths, most, q_len, q_lens):
+    """Caches that a cluster shares: sequences shorter than its warps, rows and sequences that see nothing."""
+    _run(lengths, 16, 8, 16, q_len=q_len, q_lens=q_lens, max_kv_len=most)
+
+
 def test_a_workspace_of_the_largest_call_serves_the_smaller_ones():
     ops, g = _ops(), _gen(25)
     sizes = [[ops.decode_int4_workspace_bytes(b, t, 32, 8, n) for n in (1, 64, 512, 513, 1100, 4000, 70000)]
