@@ -580,11 +580,10 @@ def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tens
     """The values held at ``slots`` as bf16 ``(key, value) [tokens, nkv, 128]``
     (``torch.ops.solort_attn.kv_load_int4``): a cached prefix for :func:`gqa_prefill`, for one. Rows
     of slot -1 are not written (undefined in tensors that this call allocates)."""
-    shape = (slots.shape[0], kv_pages.shape[1], HEAD_DIM)
-    if key is None:
-        key = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
-    if value is None:
-        value = torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device)
+    if key is None or value is None:
+        shape = (slots.shape[0], kv_pages.shape[1], HEAD_DIM)
+        key, value = (torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device) if t is None else t
+                      for t in (key, value))
     (_calls_int4.load_into if _plain(kv_pages) else _OPS.kv_load_int4)(kv_pages, slots, key, value)
     return key, value
 
