@@ -423,7 +423,7 @@ SOLORT_API int solort_attn_gemv(const SolortGemvArgs* args, void* stream);
  *
  * Slots are int64, page * P + row, on the device. -1 marks a padded row: nothing is read or written
  * for it. Any other slot outside the arena is skipped likewise and sets bit 4 of the device status.
- * Which row stays is not defined where two rows of one call have the same slot.
+ * Rows of one call must not share a slot: what it then holds is not defined.
  *
  * solort_attn_qk_norm_rope_append_int4: the attention prologue of a batch. Token i sits at
  * positions[i] of its sequence (any mix of sequences); from its row of the fused QKV projection,

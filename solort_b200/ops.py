@@ -570,7 +570,7 @@ def kv_pages_int4(num_pages: int, num_kv_heads: int, page_size: int,
 def kv_store_int4(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
                   kv_pages: torch.Tensor) -> None:
     """Hold ``key / value [tokens, nkv, 128]`` (bf16; token / head strides multiples of 8) in 4 bits at
-    ``slots`` (int64 on the device, ``page * P + row``; -1 skips a row) of ``kv_pages``
+    ``slots`` (int64 on the device, ``page * P + row``, no two alike; -1 skips a row) of ``kv_pages``
     (:func:`kv_pages_int4`; ``torch.ops.solort_attn.kv_store_int4``): the 4-bit :func:`kv_store`."""
     (_calls_int4.store_into if _plain(kv_pages) else _OPS.kv_store_int4)(key, value, slots, kv_pages)
 
