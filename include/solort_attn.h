@@ -96,6 +96,11 @@ extern "C" {
  * while that kernel is still running: the key stream then starts during its tail. Rows at q_pos[b]
  * and later (the tokens the previous kernel may just have appended), the queries and the
  * workspace are touched only after it has finished, with or without the flag.
+ * "Before" means complete when that kernel started. Stream order alone gives this where that kernel
+ * is one of the 4-bit calls below, which let the next kernel start only when all before them have
+ * finished, or was not launched by this library. The other kernels of this library let the next one
+ * start while those before them may still be running: behind one of these, the rows must have been
+ * complete earlier (an earlier graph launch, as in the runner's steps; an event; a synchronisation).
  */
 #define SOLORT_DECODE_STABLE_PREFIX 1u
 typedef struct SolortDecodeArgs {

@@ -38,9 +38,12 @@ constexpr int kTokenBytes = kBlockBytes / kBlockTokens;  // K and V of one token
 constexpr unsigned kDevErrSlot = 1u << 4;  // a slot outside the arena or a position without a RoPE row
 constexpr unsigned kDevErrPage = 1u << 5;  // a block-table entry outside the arena
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// Wait for the kernels before this one on the stream, and only then let the next one start: a kernel that
+// has started thus has finished kernels behind its predecessor. SOLORT_DECODE_STABLE_PREFIX reads before
+// the wait what those have written. Were the order the other way round, a chain of short kernels could all
+// be resident at once, and such a read could come before the write of the kernel but one.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ float lo_bf16(uint32_t u) { return __uint_as_float(u << 16); }

@@ -572,7 +572,6 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
   // low bits. Pages of 16 tokens and more: two of two blocks per tile; of 8: four.
   const uint32_t places = smem_u32(smem) + C::kOffPlaces + warp * 32 * 32;
 
-  pdl_launch_dependents();
   if (lane == 0) edge[2 * warp].u0 = edge[2 * warp + 1].u0 = -1;
   float2* unit_ml = reinterpret_cast<float2*>(smem + C::kOffUnitMl);
   if (tid < C::kRows) unit_ml[tid] = make_float2(-INFINITY, 0.f);
@@ -981,7 +980,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
   using C = Cfg<NT>;
   __shared__ float4 so[kMergeWarps][32];
   __shared__ float2 sm[kMergeWarps];
-  pdl_launch_dependents();
   if (!p.stable_prefix) pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int warps = blockDim.x >> 5;

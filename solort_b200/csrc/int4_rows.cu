@@ -89,7 +89,6 @@ __device__ __forceinline__ bool row_there(long long slot, const Arena& ar, bool 
 
 // Grid: (tokens, [query heads | key heads | value heads], p.heads each).
 __global__ void __launch_bounds__(kRowThreads, 5) append_kernel(const AppendParams p) {
-  pdl_launch_dependents();
   pdl_wait();
   const int y = blockIdx.y;
   if (y >= p.q_ctas + p.kv_ctas) {  // values: four lanes a row, two heads at a time
@@ -216,7 +215,6 @@ struct StoreParams {
 };
 
 __global__ void __launch_bounds__(kRowThreads, 8) store_kernel(const StoreParams p) {
-  pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x & 3;
   const bool is_v = static_cast<int>(blockIdx.x) >= p.nkv;  // K heads, then V heads
@@ -253,7 +251,6 @@ struct LoadParams {
 };
 
 __global__ void __launch_bounds__(kRowThreads, 16) load_kernel(const LoadParams p) {
-  pdl_launch_dependents();
   pdl_wait();
   const int l8 = threadIdx.x & 7, t = l8 & 3, g = l8 >> 2;
   const int head = blockIdx.x;

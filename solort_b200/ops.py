@@ -68,7 +68,8 @@ def gqa_decode(
     (``:250,261-263``) with ``q_len == K + 1``. ``max_kv_len`` bounds the keys read (the decode
     bucket ``bound``); it defaults to the buffer length. ``stable_prefix``: ``q_pos`` and the keys
     below it were written before the kernel launched just before this call (earlier steps), so
-    their loads may start during that kernel's tail (``SOLORT_DECODE_STABLE_PREFIX``). ``out`` and
+    their loads may start during that kernel's tail (``SOLORT_DECODE_STABLE_PREFIX`` in
+    ``include/solort_attn.h``: which kernels count as finished by then). ``out`` and
     ``workspace`` are allocated when not given (pass both to capture the call in a CUDA graph).
     """
     cap, nkv, _, _ = _static_kv(k_cache, v_cache, kv_layout)
