@@ -535,11 +535,13 @@ __device__ __forceinline__ float4 chunk_of(const Acc<NT>& A, int nt, int grp, fl
   const float inv = __uint_as_float((254u << 23) - __float_as_uint(grp & 1 ? sf.y : sf.x));
   const int c = nt / 2, e = NT > 1 ? nt & 1 : grp & 1;
   const float sum = NT > 1 ? A.xs[c][(grp >> 1) & (NT > 1)][(grp & 1) * 2 + e] : A.xs[0][0][grp];
-  const float add = pm - 7.5f * inv * sum, unit = kValueUnit * inv, unit16 = unit * 0.0625f;
+  // sum x (c - 7.5) first: 2^24 / sf would pass fp32's range for scales from 2^103 on
+  const float centre = -7.5f * sum;
   const float(&a0)[4] = A.o[c][grp][0];
   const float(&a1)[4] = A.o[c][grp][1];
-  return make_float4(fmaf(unit, a0[e], add), fmaf(unit16, a0[2 + e], add), fmaf(unit, a1[e], add),
-                     fmaf(unit16, a1[2 + e], add));
+  auto value = [&](float unit, float a) { return fmaf(inv, fmaf(unit, a, centre), pm); };
+  return make_float4(value(kValueUnit, a0[e]), value(kValueUnit * 0.0625f, a0[2 + e]), value(kValueUnit, a1[e]),
+                     value(kValueUnit * 0.0625f, a1[2 + e]));
 }
 
 // A warp's tiles of the list: from x0 on, the sequence of the first and the tiles before that. Entry
