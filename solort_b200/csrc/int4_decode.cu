@@ -16,9 +16,11 @@
 // the held scales and mids with the query's group sums (themselves split in two bf16 numbers).
 //
 // Values: a nibble in a half is an f16 subnormal, c 2^-24 or 16 c 2^-24, which costs a shift and ands
-// too and lets the other operand keep 11 bits: x = 2^8 p scale sf, with p relative to the row's running
-// maximum (at most 2^7 until that is raised) and sf the power of two that brings the group's scales
-// below 1. x is within 2^-11 of itself, and within 2^-25 below 2^-14. The codes are centred with the
+// too and lets the other operand keep 11 bits: x = p scale sf, with p relative to the row's running maximum
+// (at most 2^7 until that is raised) and sf a power of two for each row and group. sf follows the largest
+// p scale as the maximum follows the scores, up and down: a token of large values and no weight takes no bits
+// from the others. x is within 2^-11 of itself, and within 2^-25 below 2^-14, where the row's largest in the
+// group is 2^5 at least. The codes are centred with the
 // sum of the same numbers (a product with ones), O = sum x c - 7.5 sum x + sum p mid, so that their
 // rounding weighs |v - mid| and not c. p, its sum, sum p mid and all accumulators are fp32.
 //
@@ -62,10 +64,13 @@ constexpr int kDirectSteps = 6;               // the most tiles a warp takes whe
 constexpr int kSplitSteps = 2;                // what the division and its merge cost more, in tiles
 constexpr int kMostCluster = 8;               // CTAs of a cluster, the portable limit
 constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
-// A row's running maximum is raised only when a score passes it by 2^kLazy; p is 2^kPShift there, so
-// that x stays below 2^15, inside f16.
+// A row's running maximum is raised only when a score passes it by 2^kLazy, and its power of two for a group
+// is set anew only when an x of a tile could pass 2^15, inside f16: it then brings the row's largest p scale
+// into [2^kXBits, 2^(kXBits + 1)).
 constexpr float kLazy = 7.f;
-constexpr float kPShift = 15.f - kLazy;
+constexpr int kXBits = 6;
+constexpr float kMostX = 32768.f;
+constexpr int kMostSf = 127 + 119;         // exponent field of the greatest power of two: p sf stays finite
 constexpr float kCodeUnit = 512.f;         // a key code's e4m3 value is c / 512
 constexpr float kValueUnit = 16777216.f;   // a value code's f16 value is c 2^-24, or 16 c 2^-24
 
@@ -284,7 +289,7 @@ struct Acc {
   float l[NT];    // and of p
   float off[NT];  // p = 2^(score - off)
   float top[NT];  // scores above it raise the maximum
-  f2 sf[2];       // per group pair
+  f2 sf[NT][2];   // per row and group pair
 };
 
 // One tile of 32 tokens for the segment's rows; this lane's tokens are tok0 + 8 i + lane / 4 of block
@@ -363,85 +368,40 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
     }
   }
   bool raise = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-    raise |= fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3])) > A.top[nt];
-  f2 sc[4][2];  // [token][group pair] scale * sf, at most 1
-  float most = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
+  {
+    f2 wide[2];  // the largest scales of this lane's tokens (not negative: as integers; with a NaN the group is NaN)
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      sc[i][q] = mul2(pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1))), A.sf[q]);
-      const float2 v = both(sc[i][q]);
-      most = fmaxf(most, fmaxf(v.x, v.y));
-    }
-  raise |= most > 1.f;
-  if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
-    if (__any_sync(0xffffffffu, most > 1.f)) {
-      // The groups' largest scales, two bf16 bit patterns (not negative: they compare as integers) a word;
-      // a NaN does not count, it makes the sums of the rows that see it NaN by itself.
-      uint32_t top[2];
+      uint32_t w = 0;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        top[q] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = __byte_perm(word(meta[i], 2 * q), word(meta[i], 2 * q + 1), 0x5410);
-          top[q] = __vmaxu2(top[q], two & ~__vcmpgtu2(two, 0x7f7f7f7fu));
-        }
-      }
-#pragma unroll
-      for (int o = 1; o <= 16; o <<= 1) {
-        const uint32_t t0 = __shfl_xor_sync(0xffffffffu, top[0], o), t1 = __shfl_xor_sync(0xffffffffu, top[1], o);
-        top[0] = __vmaxu2(top[0], t0);
-        top[1] = __vmaxu2(top[1], t1);
-      }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float2 was = both(A.sf[q]);
-        float sf[2], f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // The power of two that brings the scale into [0.5, 1).
-          const uint32_t bits = e ? top[q] >> 16 : top[q] & 0xffffu;
-          const float old = e ? was.y : was.x;
-          const float now = __uint_as_float(static_cast<uint32_t>(max(253 - static_cast<int>(bits >> 7), 1)) << 23);
-          sf[e] = bits ? fminf(old, now) : old;
-          const int down = static_cast<int>(__float_as_uint(sf[e]) >> 23) -
-                           static_cast<int>(__float_as_uint(old) >> 23);
-          f[e] = down < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + down) << 23);  // sf / old
-        }
-        A.sf[q] = pair(sf[0], sf[1]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int c = 0; c < Acc<NT>::kCols; ++c) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) A.o[c][2 * q + e][0][i] *= f[e], A.o[c][2 * q + e][1][i] *= f[e];
-            if (NT > 1)
-              A.xs[c][q & (NT > 1)][2 * e] *= f[e], A.xs[c][q & (NT > 1)][2 * e + 1] *= f[e];
-            else
-              A.xs[c][0][2 * q + e] *= f[e];
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sc[i][q] = mul2(pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1))), A.sf[q]);
-      }
+      for (int i = 0; i < 4; ++i) w = __vmaxu2(w, __byte_perm(word(meta[i], 2 * q), word(meta[i], 2 * q + 1), 0x5410));
+      wide[q] = pair(lo_bf16(w), hi_bf16(w));
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const float mx = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
+      const float2 a = both(mul2(wide[0], A.sf[nt][0])), c = both(mul2(wide[1], A.sf[nt][1]));
+      const float most = fmaxf(fmaxf(a.x, a.y), fmaxf(c.x, c.y)) * ex2(mx - A.off[nt]);
+      raise |= mx > A.top[nt] || !(most <= kMostX);
+    }
+  }
+  if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = nt / 2, e = nt & 1;
       float mx = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
 #pragma unroll
       for (int o = 4; o <= 16; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      int up = 0;  // what is summed up has lost so many bits of weight
       if (mx > A.top[nt]) {
-        const float off = mx - kPShift, f = A.top[nt] == -INFINITY ? 0.f : ex2(A.off[nt] - off);
-        A.off[nt] = off;
+        const bool first = A.top[nt] == -INFINITY;
+        const float f = first ? 0.f : ex2(A.off[nt] - mx);
+        up = first ? 255 : static_cast<int>(fminf(mx - A.off[nt], 255.f));
+        A.off[nt] = mx;
         A.top[nt] = mx + kLazy;
         A.l[nt] *= f;
         A.pm[nt][0] = mul2(A.pm[nt][0], dup(f));
         A.pm[nt][1] = mul2(A.pm[nt][1], dup(f));
-        const int c = nt / 2, e = nt & 1;
 #pragma unroll
         for (int grp = 0; grp < 4; ++grp)
 #pragma unroll
@@ -453,6 +413,39 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
             A.xs[0][0][i] *= f;
           else if ((i & 1) == e)
             A.xs[c][0][i] *= f, A.xs[c][NT > 1][i] *= f;
+      }
+      // The exponents of the groups' largest p scale, a byte each; a NaN does not count, it makes the sums of
+      // the rows that see it NaN by itself.
+      uint32_t top = 0;
+#pragma unroll
+      for (int grp = 0; grp < 4; ++grp) {
+        float w = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w = fmaxf(w, ex2(s[nt][i] - A.off[nt]) * lo_bf16(word(meta[i], grp)));
+        top |= (__float_as_uint(w) >> 23) << (8 * grp);
+      }
+#pragma unroll
+      for (int o = 4; o <= 16; o <<= 1) top = __vmaxu4(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float2 was = both(A.sf[nt][q]);
+        float sf[2];
+#pragma unroll
+        for (int g2 = 0; g2 < 2; ++g2) {
+          const int grp = 2 * q + g2, old = static_cast<int>(__float_as_uint(g2 ? was.y : was.x) >> 23);
+          const int now = min(min(old + up, kMostSf), 254 + kXBits - static_cast<int>(top >> (8 * grp) & 255u));
+          sf[g2] = __uint_as_float(static_cast<uint32_t>(now) << 23);
+          const int by = min(127 + now - old, 254);
+          const float f = by < 1 ? 0.f : __uint_as_float(static_cast<uint32_t>(by) << 23);  // sf / old
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (NT == 1 || (i & 1) == e) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
+          if (NT > 1)
+            A.xs[c][q & (NT > 1)][2 * g2 + e] *= f;
+          else
+            A.xs[0][0][grp] *= f;
+        }
+        A.sf[nt][q] = pair(sf[0], sf[1]);
       }
     }
   }
@@ -474,9 +467,10 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const f2 mid = pair(hi_bf16(word(meta[i], 2 * q)), hi_bf16(word(meta[i], 2 * q + 1)));
+      const f2 scale = pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1)));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        x[nt][i] = mul2(dup(s[nt][i]), sc[i][q]);
+        x[nt][i] = mul2(mul2(dup(s[nt][i]), A.sf[nt][q]), scale);
         A.pm[nt][q] = fma2(dup(s[nt][i]), mid, A.pm[nt][q]);
       }
     }
@@ -530,7 +524,7 @@ __device__ __forceinline__ void write_row4(const Params& p, int b, int kvh, int 
 // This lane's chunk of its row of n8 tile nt: dims 32 grp + 4 (lane / 4) .. + 3.
 template <int NT>
 __device__ __forceinline__ float4 chunk_of(const Acc<NT>& A, int nt, int grp, float pm) {
-  const float2 sf = both(A.sf[grp >> 1]);
+  const float2 sf = both(A.sf[nt][grp >> 1]);
   // 1 / sf, a power of two
   const float inv = __uint_as_float((254u << 23) - __float_as_uint(grp & 1 ? sf.y : sf.x));
   const int c = nt / 2, e = NT > 1 ? nt & 1 : grp & 1;
@@ -804,6 +798,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
       fr[nt] = p.scale_log2 * kCodeUnit * __uint_as_float(static_cast<uint32_t>(127 - row_up) << 23);
       A.l[nt] = 0.f, A.off[nt] = 0.f, A.top[nt] = -INFINITY;
       A.pm[nt][0] = A.pm[nt][1] = 0;
+      A.sf[nt][0] = A.sf[nt][1] = dup(__uint_as_float(static_cast<uint32_t>(kMostSf) << 23));  // the first tile sets it
     }
 #pragma unroll
     for (int c = 0; c < Acc<NT>::kCols; ++c)
@@ -813,7 +808,6 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
         for (int grp = 0; grp < 4; ++grp) A.o[c][grp][0][j] = A.o[c][grp][1][j] = 0.f;
         A.xs[c][0][j] = A.xs[c][NT > 1][j] = 0.f;
       }
-    A.sf[0] = A.sf[1] = dup(__uint_as_float(253u << 23));  // the first tile sets it
     // ---- its tiles ----
     for (; x < seg_end; ++x) {
       if (__builtin_expect((issued - x0 & 31) == 0, 0)) resolve(issued);

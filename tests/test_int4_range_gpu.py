@@ -66,3 +66,84 @@ def test_values_of_every_magnitude(power, heads):
     g = _gen(power + heads)
     k, v = _randn(g, 300, 1, 128), _randn(g, 300, 1, 128).clamp(-3, 3) * 2.0 ** power
     _check(_randn(g, 1, 1, heads, 128).to(BF), *_held(g, k, v))
+
+
+def _along(n, score):
+    """Keys that score ``score`` (a number each) with queries of ones, scaled by 128^-0.5: constant rows,
+    which are held exactly where they are bf16 numbers."""
+    return (torch.as_tensor(score, device="cuda", dtype=torch.float32).expand(n) / 128 ** 0.5)[:, None, None].expand(n, 1, 128)
+
+
+def _ones(g, t, heads):
+    return (1 + 0.05 * _randn(g, 1, t, heads, 128)).to(BF)
+
+
+@pytest.mark.parametrize("heads", [2, 4, 8])
+@pytest.mark.parametrize("power", [20, 24, 28, 34, 60, 100])
+@pytest.mark.parametrize("at", [0, 333, 699])
+def test_a_token_of_large_values_and_no_weight(power, heads, at):
+    """Its scale is 2^power times the others', its weight e^-(0.7 power + 4) and less."""
+    g, n = _gen(power + heads + at), 700
+    k, v = _randn(g, n, 1, 128), _randn(g, n, 1, 128)
+    k[at] = _along(1, -0.7 * power - 12.0)[0]
+    v[at] *= 2.0 ** power
+    _check(_ones(g, 1, heads), *_held(g, k, v))
+
+
+@pytest.mark.parametrize("heads", [4, 8])
+@pytest.mark.parametrize("power", [30, 80])
+def test_a_large_token_that_half_of_the_heads_look_at(power, heads):
+    """The others' results stay their own, in a group of its own size too."""
+    g, n = _gen(power + heads), 500
+    k, v = _randn(g, n, 1, 128), _randn(g, n, 1, 128)
+    k[200] = _along(1, 60.0)[0]
+    v[200, :, :96] *= 2.0 ** power
+    q = _ones(g, 1, heads)
+    q[:, :, ::2] *= -1
+    _check(q, *_held(g, k, v))
+
+
+@pytest.mark.parametrize("score", [-45.0, 0.0, 30.0])
+@pytest.mark.parametrize("q_len,heads", [(2, 1), (2, 4), (5, 2), (4, 8)])
+def test_a_large_token_that_only_the_last_row_sees(q_len, heads, score):
+    g, n = _gen(q_len + heads), 160
+    k, v = _randn(g, n, 1, 128), _randn(g, n, 1, 128)
+    k[n - 1] = _along(1, score)[0]
+    v[n - 1] *= 2.0 ** 40
+    _check(_ones(g, q_len, heads), *_held(g, k, v))
+
+
+@pytest.mark.parametrize("heads", [2, 4, 8])
+@pytest.mark.parametrize("size", [0.0, 1e-20, 1e-3])
+@pytest.mark.parametrize("at", [0, 400, 699])
+def test_nearly_all_weight_on_a_token_of_small_values(size, heads, at):
+    """Heads that look away: the result is what the other tokens give, e^-20 of the weight each."""
+    g, n = _gen(heads + at), 700
+    k, v = _randn(g, n, 1, 128), _randn(g, n, 1, 128)
+    k[at] = _along(1, 20.0)[0]
+    v[at] *= size
+    _check(_ones(g, 1, heads), *_held(g, k, v))
+
+
+@pytest.mark.parametrize("heads", [2, 4, 8])
+@pytest.mark.parametrize("falling", [False, True])
+def test_values_that_shrink_while_scores_grow(heads, falling):
+    """From 2^60 with no weight in the end to 1 with all of it, or the other way round; the power of two of
+    a row has to follow both ways."""
+    g, n = _gen(heads), 960
+    steps = torch.linspace(0, 1, n, device="cuda")
+    steps = (1 - steps) if falling else steps
+    k = _along(n, 90 * steps) + 0.02 * _randn(g, n, 1, 128)
+    v = _randn(g, n, 1, 128) * 2.0 ** (60 * (1 - steps))[:, None, None]
+    _check(_ones(g, 1, heads), *_held(g, k, v))
+
+
+def test_broken_values_without_weight_stay_visible():
+    """A NaN in V reaches every row that sees it, whatever its weight."""
+    ops, g, n = _ops(), _gen(1), 200
+    k, v = _randn(g, n, 1, 128), _randn(g, n, 1, 128)
+    k[50], v[50] = _along(1, -200.0)[0], float("nan")
+    pages, table, _ = _held(g, k, v)
+    for heads in (4, 8):
+        out = ops.gqa_decode_paged_int4(_ones(g, 1, heads), pages, table, torch.tensor([n - 1], device="cuda"), max_kv_len=n)
+        assert out.isnan().all()
