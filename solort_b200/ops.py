@@ -548,11 +548,24 @@ def kv_store(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
 # ---- the paged KV cache held in 4 bits ----
 #
 # A decode step makes these calls once a layer, some of them shorter on the GPU than the dispatcher's
-# way round to them (about 3 us a call): on plain tensors outside a trace they go to the ops' body
-# directly.
+# way round to them (about 3 us a call): where the dispatcher would do nothing but call the op's body, they
+# call it themselves. Anything that looks on from the dispatcher (a dispatch or function mode, a transform, a
+# trace, a profiler) or that a tensor brings along (a subclass) goes through the op.
 
-def _plain(t: torch.Tensor) -> bool:
-    return type(t) is torch.Tensor and t.is_cuda and not torch.compiler.is_compiling()
+# The thread's dispatch keys with nothing of that kind at work (in inference mode only the first).
+_KEYS_AT_REST = (torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect) |
+                 torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
+_thread_keys = torch._C._dispatch_tls_local_include_set
+_function_modes = torch._C._len_torch_function_stack
+_profiled = torch._C._autograd._profiler_enabled
+_compiling = torch.compiler.is_compiling
+_PLAIN_TYPES = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+
+
+def _direct(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call with these tensors, on the device of the first, may pass the dispatcher by."""
+    return not (_compiling() or _profiled() or _function_modes() or _thread_keys().raw_repr() & ~_KEYS_AT_REST or
+                not tensors[0].is_cuda or not _PLAIN_TYPES.issuperset(map(type, tensors)))
 
 
 def kv_pages_int4(num_pages: int, num_kv_heads: int, page_size: int,
@@ -573,7 +586,8 @@ def kv_store_int4(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor,
     """Hold ``key / value [tokens, nkv, 128]`` (bf16; token / head strides multiples of 8) in 4 bits at
     ``slots`` (int64 on the device, ``page * P + row``, no two alike; -1 skips a row) of ``kv_pages``
     (:func:`kv_pages_int4`; ``torch.ops.solort_attn.kv_store_int4``): the 4-bit :func:`kv_store`."""
-    (_calls_int4.store_into if _plain(kv_pages) else _OPS.kv_store_int4)(key, value, slots, kv_pages)
+    store = _calls_int4.store_into if _direct(kv_pages, key, value, slots) else _OPS.kv_store_int4
+    store(key, value, slots, kv_pages)
 
 
 def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tensor | None = None,
@@ -585,7 +599,8 @@ def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tens
         shape = (slots.shape[0], kv_pages.shape[1], HEAD_DIM)
         key, value = (torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device) if t is None else t
                       for t in (key, value))
-    (_calls_int4.load_into if _plain(kv_pages) else _OPS.kv_load_int4)(kv_pages, slots, key, value)
+    load = _calls_int4.load_into if _direct(kv_pages, key, value, slots) else _OPS.kv_load_int4
+    load(kv_pages, slots, key, value)
     return key, value
 
 
@@ -618,7 +633,8 @@ def qk_norm_rope_append_int4(
         q_out = torch.empty(qkv.shape[0], num_qo_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
     elif q_out.dim() != 3 or q_out.shape[1] != num_qo_heads:
         raise RuntimeError(f"q_out must be [tokens, {num_qo_heads}, 128]")
-    (_calls_int4.append_into if _plain(kv_pages) else _OPS.qk_norm_rope_append_int4)(
+    direct = _direct(kv_pages, qkv, q_norm_weight, k_norm_weight, cos, sin, positions, slots, q_out)
+    (_calls_int4.append_into if direct else _OPS.qk_norm_rope_append_int4)(
         qkv, q_norm_weight, k_norm_weight, float(eps), cos, sin, positions, slots, kv_pages, q_out)
     return q_out
 
@@ -668,7 +684,8 @@ def gqa_decode_paged_int4(
                                                           int(num_ctas))
         workspace = (torch.empty(need, dtype=torch.uint8, device=q.device) if need
                      else _empty_workspace(q.device))
-    (_calls_int4.decode_into if _plain(kv_pages) else _OPS.gqa_decode_paged_int4)(
+    direct = _direct(kv_pages, q, block_table, q_pos, out, workspace, q_lens)
+    (_calls_int4.decode_into if direct else _OPS.gqa_decode_paged_int4)(
         q, kv_pages, block_table, q_pos, out, workspace, int(max_kv_len), scale, q_lens, int(num_ctas),
         bool(stable_prefix))
     return out
