@@ -459,8 +459,8 @@ typedef struct SolortInt4AppendArgs {
 
 SOLORT_API int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* args, void* stream);
 
-/* Store: token i's K and V rows (bf16, head h at + h*stride_head) to slots[i]. The 4-bit form of
- * solort_attn_kv_store (src/solort/cache/kv_cache.py:191-235). */
+/* Store: token i's K and V rows (bf16, head h at + h*stride_head) to slots[i], 2^30 tokens at most. The
+ * 4-bit form of solort_attn_kv_store (src/solort/cache/kv_cache.py:191-235). */
 typedef struct SolortInt4StoreArgs {
   const void* key;
   const void* value;

@@ -204,6 +204,9 @@ __global__ void __launch_bounds__(kRowThreads, 5) append_kernel(const AppendPara
   }
 }
 
+// Rows of a store, so that the row of a CTA's next round stays inside an int.
+constexpr int kMostStored = 1 << 30;
+
 // Eight CTAs an SM: 16380 rows 17.0 us; 17.6 with the 65 registers that the compiler takes, seven CTAs.
 struct StoreParams {
   const bf16* key;
@@ -395,6 +398,7 @@ extern "C" int solort_attn_kv_store_int4(const SolortInt4StoreArgs* a, void* str
   int rc = i4::make_arena(a->kv_pages, a->kv_stride_page, a->kv_stride_head, a->page_size,
                           a->num_pages, a->num_kv_heads, a->head_dim, a->slots, a->num_tokens, &p.ar);
   if (rc != SOLORT_OK) return rc;
+  if (a->num_tokens > i4::kMostStored) return SOLORT_ERR_UNSUPPORTED;
   if (a->num_tokens == 0) return SOLORT_OK;
   if (!a->key || !a->value) return SOLORT_ERR_INVALID_ARGUMENT;
   const int64_t strides = a->key_stride_token | a->key_stride_head | a->value_stride_token |
