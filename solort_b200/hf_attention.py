@@ -129,6 +129,11 @@ def _mirror_to_solort_kv(module: Any, key: torch.Tensor, value: torch.Tensor) ->
         return None
     kv_cache = _KV_CONTEXT["kv_cache"]
     arena = _arena_of(kv_cache)
+    if arena is not None and (arena.dim() != 6 or not arena.is_floating_point()):
+        raise RuntimeError(
+            "the bridge's paged arena must be [layers, pages, 2, P, nkv, head_dim] in 16 bits, got "
+            f"{arena.dtype} {list(arena.shape)} (the 4-bit cache has its own calls: ops.kv_store_int4, "
+            "ops.gqa_decode_paged_int4)")
     layer_idx = getattr(module, "layer_idx", None)
     slots = _KV_CONTEXT["slot_mapping"]
     ok = (layer_idx is not None and slots and arena is not None and 0 <= layer_idx < arena.shape[0]
