@@ -106,12 +106,12 @@ def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positio
                 q_out) -> None:
     """The batch attention prologue into the 4-bit cache: the body of
     ``solort_attn::qk_norm_rope_append_int4``. Head counts follow from ``q_out`` and ``kv_pages``."""
-    t = qkv.shape[0]
+    t = qkv.shape[0] if qkv.dim() else 0
     pages, cs, outs = kv_pages.shape, cos.shape, q_out.shape
     index = qkv.get_device()
     sp, so, sc, sx = kv_pages.stride(), q_out.stride(), cos.stride(), qkv.stride()
-    P = pages[-1] // TOKEN_BYTES
-    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+    P = pages[2] // TOKEN_BYTES if len(pages) == 3 else 0
+    if not (P >= 8 and not P & (P - 1) and sp[2] == 1 and kv_pages.dtype is _U8 and
             P * TOKEN_BYTES == pages[2] and len(outs) == 3 and len(cs) == 2 and index >= 0 and
             index == kv_pages.get_device() == q_out.get_device() == cos.get_device() ==
             sin.get_device() == positions.get_device() == slots.get_device() ==
@@ -150,8 +150,8 @@ def append_into(qkv, q_norm_weight, k_norm_weight, eps: float, cos, sin, positio
 def _key_value(call, key, value, slots, kv_pages) -> None:
     pages, sp = kv_pages.shape, kv_pages.stride()
     sk, sv, index, n = key.stride(), value.stride(), key.get_device(), slots.numel()
-    P = pages[-1] // TOKEN_BYTES
-    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+    P = pages[2] // TOKEN_BYTES if len(pages) == 3 else 0
+    if not (P >= 8 and not P & (P - 1) and sp[2] == 1 and kv_pages.dtype is _U8 and
             P * TOKEN_BYTES == pages[2] and index >= 0 and
             index == value.get_device() == slots.get_device() == kv_pages.get_device() and
             _BF16 is key.dtype is value.dtype and slots.dtype is _I64 and slots.shape == (n,) and
@@ -181,8 +181,8 @@ def decode_fields(q, kv_pages, block_table, q_pos, out, max_kv_len: int, scale: 
     """The device index and the checked fields of a decode call before its workspace."""
     shape, pages, table, st = q.shape, kv_pages.shape, block_table.shape, block_table.stride()
     sq, so, sp, index = q.stride(), out.stride(), kv_pages.stride(), q.get_device()
-    P = pages[-1] // TOKEN_BYTES
-    if not (len(pages) == 3 and sp[2] == 1 and kv_pages.dtype is _U8 and P >= 8 and not P & (P - 1) and
+    P = pages[2] // TOKEN_BYTES if len(pages) == 3 else 0
+    if not (P >= 8 and not P & (P - 1) and sp[2] == 1 and kv_pages.dtype is _U8 and
             P * TOKEN_BYTES == pages[2] and len(shape) == 4 and len(table) == 2 and index >= 0 and
             index == kv_pages.get_device() == block_table.get_device() == q_pos.get_device() ==
             out.get_device() and _BF16 is q.dtype is out.dtype and block_table.dtype is _I32 and

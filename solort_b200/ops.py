@@ -596,7 +596,8 @@ def kv_load_int4(kv_pages: torch.Tensor, slots: torch.Tensor, *, key: torch.Tens
     (``torch.ops.solort_attn.kv_load_int4``): a cached prefix for :func:`gqa_prefill`, for one. Rows
     of slot -1 are not written (undefined in tensors that this call allocates)."""
     if key is None or value is None:
-        shape = (slots.shape[0], kv_pages.shape[1], HEAD_DIM)
+        _calls_int4.page_size(kv_pages)
+        shape = (slots.numel(), kv_pages.shape[1], HEAD_DIM)
         key, value = (torch.empty(shape, dtype=torch.bfloat16, device=kv_pages.device) if t is None else t
                       for t in (key, value))
     load = _calls_int4.load_into if _direct(kv_pages, key, value, slots) else _OPS.kv_load_int4
@@ -627,9 +628,11 @@ def qk_norm_rope_append_int4(
     or any mix. A token of slot -1 (a padded row of a captured batch) is skipped, its ``q_out`` row
     too. ``cos``/``sin`` as in :func:`qk_norm_rope_append`. Norm and rotation are fp32 with one
     rounding at the end."""
-    if kv_pages.shape[1] != num_kv_heads:
-        raise RuntimeError(f"kv_pages has {kv_pages.shape[1]} KV heads, not {num_kv_heads}")
+    if kv_pages.dim() != 3 or kv_pages.shape[1] != num_kv_heads:
+        raise RuntimeError(f"kv_pages {list(kv_pages.shape)} is not an arena of {num_kv_heads} KV heads")
     if q_out is None:
+        if qkv.dim() != 2:
+            raise RuntimeError(f"qkv must be [tokens, ({num_qo_heads} + 2 * {num_kv_heads}) * 128]")
         q_out = torch.empty(qkv.shape[0], num_qo_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
     elif q_out.dim() != 3 or q_out.shape[1] != num_qo_heads:
         raise RuntimeError(f"q_out must be [tokens, {num_qo_heads}, 128]")
