@@ -496,9 +496,11 @@ SOLORT_API int solort_attn_kv_load_int4(const SolortInt4LoadArgs* args, void* st
  * more). Rows that see no key are zero; rows past q_lens are not written. Keys behind a block-table entry outside the arena
  * count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
  * elements; out 8-byte aligned, multiples of 4. The workspace (256-byte aligned; query its size with
- * the same args) is 0 for short caches, else two partial results a CTA of one resident wave and 8 bytes
- * per sequence, KV head and row block; it never shrinks as batch, q_len or max_kv_len grow, so one for
- * the largest call serves the smaller ones. Nothing in it outlives a call; calls that share one must be
+ * the same args) is 0 for caches of up to 512 keys whose units (sequence, KV head, row block) are all
+ * resident at once, else two partial results a CTA of one resident wave and 8 bytes per unit. At given
+ * head counts and num_ctas it never shrinks as batch, q_len or max_kv_len grow, so one for the largest
+ * call serves the smaller ones; other head counts need a query of their own, and fewer heads may need
+ * more. Nothing in it outlives a call; calls that share one must be
  * ordered on their streams. num_ctas: 0 = one resident wave, otherwise the number of CTAs over which
  * the keys are divided.
  */

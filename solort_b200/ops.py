@@ -645,8 +645,10 @@ def qk_norm_rope_append_int4(
 def decode_int4_workspace_bytes(batch: int, q_len: int, num_qo_heads: int, num_kv_heads: int,
                                 max_kv_len: int, *, num_ctas: int = 0) -> int:
     """Workspace bytes a :func:`gqa_decode_paged_int4` call with these sizes needs on the current
-    device: 0 for short caches, else some MiB and 8 bytes per sequence, KV head and block of 8 rows. It
-    never shrinks as a size grows, so a workspace of the largest call serves the smaller ones."""
+    device: 0 for caches of up to 512 keys whose units (sequence, KV head, block of 4 or 8 rows) are all
+    resident at once, else some MiB and 8 bytes per unit. At given head counts it never shrinks as
+    ``batch``, ``q_len`` or ``max_kv_len`` grows, so a workspace of the largest call serves the smaller
+    ones; for several models on one workspace, take the greatest of their sizes."""
     return _calls_int4.decode_workspace_bytes(batch, q_len, num_qo_heads, num_kv_heads, max_kv_len,
                                               num_ctas)
 
