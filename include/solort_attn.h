@@ -493,8 +493,8 @@ SOLORT_API int solort_attn_kv_load_int4(const SolortInt4LoadArgs* args, void* st
  * GQA attention of q_len query tokens per sequence over the 4-bit pages: solort_attn_decode with a
  * block table (q, out, q_pos, q_lens, max_kv_len, block_table and the SOLORT_DECODE_STABLE_PREFIX
  * flag as there), for any q_len: the rows of a KV head are taken in blocks of 8 (4 where there are no
- * more). Rows that see no key are zero; rows past q_lens are not written. Keys behind a block-table entry outside the arena
- * count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
+ * more), and max_kv_len of 2^30 at most. Rows that see no key are zero; rows past q_lens are not written.
+ * Keys behind a block-table entry outside the arena count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
  * elements; out 8-byte aligned, multiples of 4. The workspace (256-byte aligned; query its size with
  * the same args) is 0 for caches of up to 512 keys whose units (sequence, KV head, row block) are all
  * resident at once, else two partial results a CTA of one resident wave and 8 bytes per unit. At given

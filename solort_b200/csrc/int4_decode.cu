@@ -63,6 +63,7 @@ constexpr int kUnitCost = 4;                  // tiles' worth of set-up of a uni
 constexpr int kDirectSteps = 6;               // the most tiles a warp takes where the list is not divided
 constexpr int kSplitSteps = 2;                // what the division and its merge cost more, in tiles
 constexpr int kMostCluster = 8;               // CTAs of a cluster, the portable limit
+constexpr int kMostKeys = 1 << 30;            // keys of a sequence
 constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
 // A row's running maximum is raised only when a score passes it by 2^kLazy, and its power of two for a group
 // is set anew only when an x of a tile could pass 2^15, inside f16: it then brings the row's largest p scale
@@ -1064,9 +1065,10 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   const int64_t tiles = (static_cast<int64_t>(a->max_kv_len) + kTile - 1) / kTile + kUnitCost;
   const int64_t units = rb * a->num_kv_heads;
   const int64_t out_rows = static_cast<int64_t>(a->batch) * a->q_len * a->num_qo_heads;
-  const int64_t limit = (1ll << 31) - 1;
-  if (rows > limit || units > limit || out_rows > limit || tiles > limit / units ||
-      tiles * units > limit / a->batch)
+  // Tokens, and places in the list, stay inside an int with a tile, or a CTA's warps, added to them.
+  const int64_t limit = (1ll << 31) - 1, most_listed = 1ll << 30;
+  if (rows > limit || units > limit || out_rows > limit || a->max_kv_len > kMostKeys ||
+      tiles > most_listed / units || tiles * units > most_listed / a->batch)
     return SOLORT_ERR_UNSUPPORTED;
   DeviceInfo di;
   int rc = current_device_info(&di);
