@@ -63,6 +63,7 @@ constexpr int kUnitCost = 4;                  // tiles' worth of set-up of a uni
 constexpr int kDirectSteps = 6;               // the most tiles a warp takes where the list is not divided
 constexpr int kSplitSteps = 2;                // what the division and its merge cost more, in tiles
 constexpr int kMostCluster = 8;               // CTAs of a cluster, the portable limit
+constexpr int kApartTiles = 128;              // tiles of a warp from which eight rows' sums of a tile stay apart
 constexpr int kMostKeys = 1 << 30;            // keys of a sequence
 constexpr int kBareTiles = 16;                // up to this many tiles a unit may go without a workspace
 // A row's running maximum is raised only when a score passes it by 2^kLazy, and its power of two for a group
@@ -256,13 +257,27 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// d += a b, m16n8k16 f16.
+// d = a b, and d += a b, m16n8k16 f16.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void add4(float (&d)[4], const float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float2 r = both(add2(pair(d[i], d[i + 1]), pair(v[i], v[i + 1])));
+    d[i] = r.x, d[i + 1] = r.y;
+  }
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
@@ -281,8 +296,9 @@ struct Acc {
   static constexpr int kCols = NT > 1 ? NT / 2 : 1;  // n8 tiles of the second product
   // [tile][group][m16 tile h]: c0, c1 dim 32 g + 4 (lane / 4) + 2 h, c2, c3 the dim after. The columns
   // are two rows (nt = 2 tile, 2 tile + 1), or with one row a lane that row for the two groups of a
-  // pair, of which the one is the group's own and the other is waste.
-  float o[kCols][4][2][4];
+  // pair, of which the group's own is kept.
+  static constexpr int kKept = NT > 1 ? 4 : 2;
+  float o[kCols][4][2][kKept];
   // Sums of x: [tile][group pair], columns of the even group in c0, c1 and of the odd in c2, c3; with
   // one row a lane [0][0], of the pair 0 and 1.
   float xs[kCols][NT > 1 ? 2 : 1][4];
@@ -295,7 +311,7 @@ struct Acc {
 
 // One tile of 32 tokens for the segment's rows; this lane's tokens are tok0 + 8 i + lane / 4 of block
 // i. `masked`: some row does not see some token; `there` has a bit for each block that was loaded.
-template <int NT>
+template <int NT, bool kApart>
 __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT][4][2],
                                           const uint32_t (&qm)[NT][2], Acc<NT>& A, const float (&fr)[NT],
                                           bool masked, const int (&lim)[NT], int tok0, unsigned there) {
@@ -406,7 +422,7 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
 #pragma unroll
         for (int grp = 0; grp < 4; ++grp)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < Acc<NT>::kKept; ++i)
             if (NT == 1 || (i & 1) == e) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -439,7 +455,7 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
           const int by = min(127 + now - old, 254);
           const float f = by < 1 ? 0.f : __uint_as_float(static_cast<uint32_t>(by) << 23);  // sf / old
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < Acc<NT>::kKept; ++i)
             if (NT == 1 || (i & 1) == e) A.o[c][grp][0][i] *= f, A.o[c][grp][1][i] *= f;
           if (NT > 1)
             A.xs[c][q & (NT > 1)][2 * g2 + e] *= f;
@@ -490,11 +506,31 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
         }
       }
     }
+    // Sums of x and of x c over the tile: into the running ones, or apart and then added to them.
+    float sum[2][Acc<NT>::kCols][2][4], ones_sum[Acc<NT>::kCols][4];
+    auto product = [&](float(&part)[4], auto& all, const uint32_t(&a4)[4], uint32_t b0, uint32_t b1, bool first) {
+      if constexpr (!kApart)
+        mma_f16(all, a4, b0, b1);
+      else if (first)
+        mma_f16_first(part, a4, b0, b1);
+      else
+        mma_f16(part, a4, b0, b1);
+    };
+#pragma unroll
+    for (int c = 0; c < Acc<NT>::kCols; ++c)
+#pragma unroll
+      for (int e = 0; e < (NT > 1 ? 2 : 1); ++e) {
+        // rows 0..7 of ones add up the first of two groups, or pairs, and rows 8..15 the second
+        const bool second = NT > 1 ? e : q;
+        const uint32_t lo_rows = second ? 0u : kOnes, hi_rows = second ? kOnes : 0u;
+        const uint32_t ones[4] = {lo_rows, hi_rows, lo_rows, hi_rows};
+#pragma unroll
+        for (int k = 0; k < 4; k += 2)
+          product(ones_sum[c], A.xs[c][q & (NT > 1)], ones, bb[e][c][k], bb[e][c][k + 1], e + k == 0);
+      }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int grp = 2 * q + e;
-      const uint32_t lo_rows = (NT > 1 ? e : q) ? 0u : kOnes, hi_rows = (NT > 1 ? e : q) ? kOnes : 0u;
-      const uint32_t ones[4] = {lo_rows, hi_rows, lo_rows, hi_rows};
 #pragma unroll
       for (int k = 0; k < 4; k += 2) {  // tokens of blocks k, k + 1
         const uint32_t w0 = word(v[k], grp), w1 = word(v[k + 1], grp), y0 = w0 >> 8, y1 = w1 >> 8;
@@ -502,13 +538,25 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
         const uint32_t a1[4] = {y0 & kLow, y0 & kHigh, y1 & kLow, y1 & kHigh};
 #pragma unroll
         for (int c = 0; c < Acc<NT>::kCols; ++c) {
-          mma_f16(A.o[c][grp][0], a0, bb[e][c][k], bb[e][c][k + 1]);
-          mma_f16(A.o[c][grp][1], a1, bb[e][c][k], bb[e][c][k + 1]);
-          if (NT > 1)
-            mma_f16(A.xs[c][q & (NT > 1)], ones, bb[e][c][k], bb[e][c][k + 1]);
-          else if (e == 0)
-            mma_f16(A.xs[c][0], ones, bb[e][c][k], bb[e][c][k + 1]);
+          product(sum[e][c][0], A.o[c][grp][0], a0, bb[e][c][k], bb[e][c][k + 1], k == 0);
+          product(sum[e][c][1], A.o[c][grp][1], a1, bb[e][c][k], bb[e][c][k + 1], k == 0);
         }
+      }
+    }
+    if constexpr (kApart) {
+#pragma unroll
+      for (int c = 0; c < Acc<NT>::kCols; ++c) {
+        add4(A.xs[c][q & (NT > 1)], ones_sum[c]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float(&o)[Acc<NT>::kKept] = A.o[c][2 * q + e][h];
+            if constexpr (NT > 1)
+              add4(o, sum[e][c][h]);
+            else
+              o[0] += sum[e][c][h][e], o[1] += sum[e][c][h][2 + e];
+          }
       }
     }
   }
@@ -532,11 +580,13 @@ __device__ __forceinline__ float4 chunk_of(const Acc<NT>& A, int nt, int grp, fl
   const float sum = NT > 1 ? A.xs[c][(grp >> 1) & (NT > 1)][(grp & 1) * 2 + e] : A.xs[0][0][grp];
   // sum x (c - 7.5) first: 2^24 / sf would pass fp32's range for scales from 2^103 on
   const float centre = -7.5f * sum;
-  const float(&a0)[4] = A.o[c][grp][0];
-  const float(&a1)[4] = A.o[c][grp][1];
+  constexpr int kKept = Acc<NT>::kKept;
+  const float(&a0)[kKept] = A.o[c][grp][0];
+  const float(&a1)[kKept] = A.o[c][grp][1];
+  const int i0 = NT > 1 ? e : 0, i1 = NT > 1 ? 2 + e : 1;
   auto value = [&](float unit, float a) { return fmaf(inv, fmaf(unit, a, centre), pm); };
-  return make_float4(value(kValueUnit, a0[e]), value(kValueUnit * 0.0625f, a0[2 + e]), value(kValueUnit, a1[e]),
-                     value(kValueUnit * 0.0625f, a1[2 + e]));
+  return make_float4(value(kValueUnit, a0[i0]), value(kValueUnit * 0.0625f, a0[i1]), value(kValueUnit, a1[i0]),
+                     value(kValueUnit * 0.0625f, a1[i1]));
 }
 
 // A warp's tiles of the list: from x0 on, the sequence of the first and the tiles before that. Entry
@@ -549,7 +599,13 @@ struct Edge {
   int u0, u1, seq, head, row0, live;
 };
 
-template <int NT>
+// kApart: the tensor cores add up the products of a tile, and the tiles' sums are added here, in fp32 with
+// rounding to nearest. A tensor core's own running sum is cut off, for codes always downwards: of 131072 keys
+// with 8 KV heads in one CTA's warps (5461 tiles each) that was 1.13 % of the result, and 0.06 % so; at 125
+// tiles a warp the two are alike (0.03 %, of which 0.02 are the probabilities' f16 rounding). Four rows keep
+// half of the sums and gain registers; eight rows pay 6 % of a tile (8 sequences of 5 rows, 4099 keys: 29.0
+// us, 27.2 without), and have it only where a warp's tiles may be more than kApartTiles.
+template <int NT, bool kApart>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
   using C = Cfg<NT>;
   constexpr int kWarps = C::kWarps, kDepth = C::kDepth;
@@ -806,7 +862,8 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int grp = 0; grp < 4; ++grp) A.o[c][grp][0][j] = A.o[c][grp][1][j] = 0.f;
+        for (int grp = 0; grp < 4; ++grp)
+          if (j < Acc<NT>::kKept) A.o[c][grp][0][j] = A.o[c][grp][1][j] = 0.f;
         A.xs[c][0][j] = A.xs[c][NT > 1][j] = 0.f;
       }
     // ---- its tiles ----
@@ -828,7 +885,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode
           lim[nt] = r < s.rows ? static_cast<int>(max(last, -1ll)) : -1;
         }
       }
-      tile_step<NT>(ring + slot * kTileBytes, qf, qm, A, fr, masked, lim, tok, there);
+      tile_step<NT, kApart>(ring + slot * kTileBytes, qf, qm, A, fr, masked, lim, tok, there);
       __syncwarp();
     }
 
@@ -1044,7 +1101,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Params p)
 
 struct Plan {
   int nt = 1, ctas = 1, rb = 1, cluster = 1;
-  bool direct = false;
+  bool direct = false, apart = false;
   size_t o_bytes = 0, ml_bytes = 0, ws_bytes = 0;
 };
 
@@ -1101,6 +1158,7 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   // The workspace never shrinks as a size grows: one for the largest call serves the smaller ones.
   if (pl->direct && bare) return SOLORT_OK;
   pl->ctas = static_cast<int>(most < wave ? most : wave);
+  pl->apart = !pl->direct && tiles * units * a->batch > static_cast<int64_t>(kApartTiles) * pl->ctas * warps;
   const size_t parts = static_cast<size_t>(2) * pl->ctas * 4 * pl->nt;
   pl->o_bytes = parts * kHD * 4;
   pl->ml_bytes = parts * 8;
@@ -1125,16 +1183,16 @@ inline cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, void* 
   return cfg;
 }
 
-template <int NT>
+template <int NT, bool kApart>
 int launch(const Params& prm, const Plan& pl, void* stream) {
   using C = Cfg<NT>;
   static std::atomic<unsigned> configured{0};  // one bit per device ordinal < 32
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return SOLORT_ERR_CUDA;
   if (dev >= 32 || !(configured.load(std::memory_order_acquire) & (1u << dev))) {
-    if (cudaFuncSetAttribute(decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+    if (cudaFuncSetAttribute(decode_kernel<NT, kApart>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
             cudaSuccess ||
-        cudaFuncSetAttribute(decode_kernel<NT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+        cudaFuncSetAttribute(decode_kernel<NT, kApart>, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return SOLORT_ERR_CUDA;
     if (dev < 32) configured.fetch_or(1u << dev, std::memory_order_release);
@@ -1142,7 +1200,7 @@ int launch(const Params& prm, const Plan& pl, void* stream) {
   cudaLaunchAttribute attr[2];
   const dim3 grid = pl.direct ? dim3(prm.nkv * pl.rb * pl.cluster, prm.batch) : dim3(pl.ctas);
   cudaLaunchConfig_t cfg = pdl_config(grid, C::kThreads, C::kSmem, stream, pl.cluster, attr);
-  if (cudaLaunchKernelEx(&cfg, decode_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, decode_kernel<NT, kApart>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   int rc = launch_status();
   if (rc != SOLORT_OK || pl.direct) return rc;
   // Few rows have many parts each and want many warps (131072 keys, 32 rows: 8 warps 38.9 us, 2 warps
@@ -1238,5 +1296,7 @@ extern "C" int solort_attn_decode_int4(const SolortInt4DecodeArgs* a, void* stre
   p.rb = pl.rb;
   p.stable_prefix = (a->flags & SOLORT_DECODE_STABLE_PREFIX) ? 1 : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  return pl.nt == 1 ? i4::launch<1>(p, pl, stream) : i4::launch<2>(p, pl, stream);
+  return pl.nt == 1 ? i4::launch<1, true>(p, pl, stream)
+         : pl.apart ? i4::launch<2, true>(p, pl, stream)
+                    : i4::launch<2, false>(p, pl, stream);
 }
