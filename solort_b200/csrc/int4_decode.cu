@@ -20,9 +20,13 @@
 // (at most 2^7 until that is raised) and sf a power of two for each row and group. sf follows the largest
 // p scale as the maximum follows the scores, up and down: a token of large values and no weight takes no bits
 // from the others. x is within 2^-11 of itself, and within 2^-25 below 2^-14, where the row's largest in the
-// group is 2^5 at least. The codes are centred with the
-// sum of the same numbers (a product with ones), O = sum x c - 7.5 sum x + sum p mid, so that their
-// rounding weighs |v - mid| and not c. p, its sum, sum p mid and all accumulators are fp32.
+// group is 2^5 at least. The codes are centred with the sum of the same numbers (a product with ones),
+// O = sum x c - 7.5 sum x + sum p mid, so that their rounding weighs |v - mid| and not c. Tokens of a tile's
+// second and fourth blocks enter as -x times 15 - c, which centres to the same x (c - 7.5): the tensor cores cut
+// products off at a distance from the nominal exponent of the largest, and a subnormal's nominal exponent lies
+// 6 to 10 bits above a nibble in the lowest bits, 2 to 6 above one in the next. With one sign that was a bias
+// of 1e-5 of the values in every other dim, 0.05 % of the result at 131072 keys; with both it cancels (0.02 %,
+// the f16 rounding), and the sums stay small. p, its sum, sum p mid and all accumulators are fp32.
 //
 // Both products are transposed, S^T = K Q^T and O^T = V^T P^T (tokens or dims as the 16 rows), so that
 // four query rows fill an n8 tile of the first and a row pair a column pair of the second; P^T turns into
@@ -299,7 +303,7 @@ struct Acc {
   // pair, of which the group's own is kept.
   static constexpr int kKept = NT > 1 ? 4 : 2;
   float o[kCols][4][2][kKept];
-  // Sums of x: [tile][group pair], columns of the even group in c0, c1 and of the odd in c2, c3; with
+  // Sums of +-x: [tile][group pair], columns of the even group in c0, c1 and of the odd in c2, c3; with
   // one row a lane [0][0], of the pair 0 and 1.
   float xs[kCols][NT > 1 ? 2 : 1][4];
   f2 pm[NT][2];   // this lane's tokens' sum of p mid, a group pair each
@@ -487,7 +491,7 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
       const f2 scale = pair(lo_bf16(word(meta[i], 2 * q)), lo_bf16(word(meta[i], 2 * q + 1)));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        x[nt][i] = mul2(mul2(dup(s[nt][i]), A.sf[nt][q]), scale);
+        x[nt][i] = mul2(mul2(dup(i & 1 ? -s[nt][i] : s[nt][i]), A.sf[nt][q]), scale);
         A.pm[nt][q] = fma2(dup(s[nt][i]), mid, A.pm[nt][q]);
       }
     }
@@ -506,7 +510,8 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
         }
       }
     }
-    // Sums of x and of x c over the tile: into the running ones, or apart and then added to them.
+    // Sums of +-x and of their products with c or 15 - c over the tile: into the running ones, or apart and then
+    // added to them.
     float sum[2][Acc<NT>::kCols][2][4], ones_sum[Acc<NT>::kCols][4];
     auto product = [&](float(&part)[4], auto& all, const uint32_t(&a4)[4], uint32_t b0, uint32_t b1, bool first) {
       if constexpr (!kApart)
@@ -534,8 +539,8 @@ __device__ __forceinline__ void tile_step(uint32_t base, const uint32_t (&qf)[NT
 #pragma unroll
       for (int k = 0; k < 4; k += 2) {  // tokens of blocks k, k + 1
         const uint32_t w0 = word(v[k], grp), w1 = word(v[k + 1], grp), y0 = w0 >> 8, y1 = w1 >> 8;
-        const uint32_t a0[4] = {w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh};
-        const uint32_t a1[4] = {y0 & kLow, y0 & kHigh, y1 & kLow, y1 & kHigh};
+        const uint32_t a0[4] = {w0 & kLow, w0 & kHigh, ~w1 & kLow, ~w1 & kHigh};
+        const uint32_t a1[4] = {y0 & kLow, y0 & kHigh, ~y1 & kLow, ~y1 & kHigh};
 #pragma unroll
         for (int c = 0; c < Acc<NT>::kCols; ++c) {
           product(sum[e][c][0], A.o[c][grp][0], a0, bb[e][c][k], bb[e][c][k + 1], k == 0);

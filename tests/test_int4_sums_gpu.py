@@ -64,3 +64,34 @@ def test_means_of_many_values(heads, n, ctas):
     print(f"{worst:.3g} of the tolerance")
     assert worst <= 1, f"{worst:.3g} of the tolerance"
     assert ops.device_status() == 0
+
+
+def test_no_bias_in_any_place_of_a_code():
+    """The mean error over the dims of one place in a half word, over 8 heads, against eight deviations of it: an
+    element's is 2^-11 / sqrt(3) sqrt(sum p^2 (v - mid)^2) from f16 and 2^-10 sqrt(sum p^2 v^2) from its scores
+    (|q| scale <= 8), dims are independent of each other but for the two or three nibbles of a group that share
+    the f16 rounding, times factors (v - mid) of either sign."""
+    from solort_b200 import ops
+
+    g, P, n, heads, ctas = torch.Generator("cuda").manual_seed(7), 64, 1 << 19, 8, 60
+    pages = ops.kv_pages_int4(n // P, 1, P)
+    k, v = (torch.randn(n, 1, 128, generator=g, device="cuda").to(BF) for _ in "kv")
+    at = torch.arange(n, device="cuda")
+    ops.kv_store_int4(k, v, at, pages)
+    q = (torch.randn(1, 1, heads, 128, generator=g, device="cuda") * 1.5).to(BF)  # weights e^(1.5 x), x normal
+    ws = torch.zeros(ops.decode_int4_workspace_bytes(1, 1, heads, 1, n, num_ctas=ctas), dtype=U8, device="cuda")
+    ops.gqa_decode_paged_int4(q, pages, (at[:n // P]).to(I32)[None], torch.tensor([n - 1], device="cuda"), max_kv_len=n,
+                              num_ctas=ctas, workspace=ws)
+    torch.cuda.synchronize()
+    o = ws[:2 * ctas * 8 * 512].view(torch.float32).view(2 * ctas, 8, 128)[::2].double()
+    ml = ws[2 * ctas * 8 * 512:][:2 * ctas * 8 * 8].view(torch.float32).view(2 * ctas, 8, 2)[::2].double()
+    w = (ml[..., :1] - ml[..., :1].amax(0)).exp2()
+    got = (o * w).sum(0) / (ml[..., 1:] * w).sum(0)
+    hk, hv, mid = (x[:, 0] for x in Q.load(pages, at, mids=True))
+    p = torch.softmax(q[0, 0].double() @ hk.T * 128 ** -0.5, -1)
+    off = (got - p @ hv).view(heads, 32, 4)
+    each = 2.0 ** -11 / 3 ** 0.5 * (p ** 2 @ (hv - mid) ** 2).sqrt() + 2.0 ** -10 * (p ** 2 @ hv ** 2).sqrt()
+    tol = 8 * each.view(heads, 32, 4).square().mean((0, 1)).sqrt() / (heads * 32) ** 0.5
+    mean = off.mean((0, 1))
+    print(mean.tolist(), tol.tolist())
+    assert (mean.abs() <= tol).all()
