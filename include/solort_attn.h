@@ -426,8 +426,8 @@ SOLORT_API int solort_attn_gemv(const SolortGemvArgs* args, void* stream);
  *   bytes 1152..1279  the values' scale and mid, as the keys'
  * No byte is shared by two tokens. An arena of zero bytes holds zeros.
  *
- * Slots are int64, page * P + row, on the device. -1 marks a padded row: nothing is read or written
- * for it. Any other slot outside the arena is skipped likewise and sets bit 4 of the device status.
+ * Slots are int64, page * P + row, on the device. -1 marks a padded row: nothing is written for it, and
+ * what its source rows hold has no effect (they may be read). Any other slot outside the arena is skipped likewise and sets bit 4 of the device status.
  * Rows of one call must not share a slot: what it then holds is not defined.
  *
  * solort_attn_qk_norm_rope_append_int4: the attention prologue of a batch. Token i sits at
@@ -494,7 +494,10 @@ SOLORT_API int solort_attn_kv_load_int4(const SolortInt4LoadArgs* args, void* st
  * block table (q, out, q_pos, q_lens, max_kv_len, block_table and the SOLORT_DECODE_STABLE_PREFIX
  * flag as there), for any q_len: the rows of a KV head are taken in blocks of 8 (4 where there are no
  * more), and max_kv_len of 2^30 at most. Rows that see no key are zero; rows past q_lens are not written.
- * Keys behind a block-table entry outside the arena count as absent and set bit 5 of the device status. q 16-byte aligned with strides multiples of 8
+ * Keys behind a block-table entry outside the arena count as absent and set bit 5 of the device status.
+ * Sums are fp32 over weights of up to 2^7, so the result is finite while 2^7 times the number of keys times
+ * the largest value stays below 2^128 (2^17 keys: values up to 2^104); values of any two sizes may meet. A
+ * weight below 2^-126 of its row's largest counts as zero. q 16-byte aligned with strides multiples of 8
  * elements; out 8-byte aligned, multiples of 4. The workspace (256-byte aligned; query its size with
  * the same args) is 0 for caches of up to 512 keys whose units (sequence, KV head, row block) are all
  * resident at once, else two partial results a CTA of one resident wave and 8 bytes per unit. At given

@@ -35,17 +35,18 @@
 // Work split: the cache's 32-token tiles, over all sequences, KV heads and blocks of query rows, are one
 // list, divided evenly over all warps of the GPU, so that sequences of any lengths load every SM alike. A
 // unit (a sequence's KV head and row block) counts kUnitCost tiles more for its set-up: 48 sequences of
-// 127 to 8111 keys take 34.9 us with 2, 34.3 with 4, 35.2 with 8. A warp has a ring of kDepth tiles of its
+// 127 to 8111 keys take 35.5 us with 2, 35.4 with 4, 36.6 with 8. A warp has a ring of kDepth tiles of its
 // own (5120 bytes a tile, in 16-byte asynchronous copies), so warps meet only when a unit that they share
 // ends. A unit that lies within a CTA is added up there; parts of several CTAs meet in merge_kernel,
 // through `span`. Lengths are read on the device. Short caches skip the division: a unit is a CTA, or a
 // cluster of CTAs that add up their sums over shared memory (make_plan).
 //
-// Bound by memory for up to four rows: 32 query heads over 8 KV heads, 131072 keys 38.3 us (4.4 TB/s; 5.8
-// TB/s for each key beyond 16384, of 6.57 measured for a copy). The rest is what every call pays, 6.8 us
+// Bound by memory for up to four rows: 32 query heads over 8 KV heads, 131072 keys 38.8 us (4.3 TB/s; 5.6
+// TB/s for each key beyond 16384, of 6.57 measured for a copy). The rest is what every call pays, 6.5 us
 // at 1000 keys: the way of the query rows into operands, a first tile that nothing hides, the sums of the
 // parts and the cluster's barriers, or the merge's launch. Blocks of eight rows are bound by the
-// instructions of a tile, 771 a warp, 60 of them matrix products: 8 sequences of 5 rows, 4099 keys 26.3 us.
+// instructions of a tile, 810 a warp (605 for four rows), 60 of them on the matrix pipe: 8 sequences of 5
+// rows, 4099 keys 27.5 us. Probabilities are ex2.approx's, within 2^-22 of themselves.
 //
 // Reference semantics: src/solort/model/cuda_graph_executor.py:168,180-184 (keys 0..pos), :250
 // (query i at vpos0 + i), src/solort/cache/kv_cache.py:136-149 (slot = bt[pos // P] * P + pos % P).
@@ -81,9 +82,10 @@ constexpr float kCodeUnit = 512.f;         // a key code's e4m3 value is c / 512
 constexpr float kValueUnit = 16777216.f;   // a value code's f16 value is c 2^-24, or 16 c 2^-24
 
 // NT n8 tiles of four query rows each; two CTAs of six warps share an SM, 168 registers a thread. A third
-// tile in the ring, which fits for four rows, gains nothing (131072 keys 39.0 us, 38.3 without). For eight
-// rows (8 sequences of 5 rows, 4099 keys 26.5 us) eight warps of 255 registers are as fast; ten warps load
-// the four schedulers unevenly (30.3 us); sixteen rows a block want 255 registers and spill (32.9 us).
+// tile in the ring, which fits for four rows, takes longer (131072 keys 40.2 us, 38.8 without). Eight rows
+// spill a little (192 bytes of stores and 80 of loads a thread, 220 and 108 with kApart), and on 8 sequences
+// of 5 rows, 4099 keys, eight warps of 255 registers without spills are no faster; ten warps load the four
+// schedulers unevenly (14 % slower); sixteen rows in one warp want 255 registers and spill (24 % slower).
 template <int NT>
 struct Cfg {
   static constexpr int kWarps = 6;
@@ -103,7 +105,7 @@ struct Cfg {
   static constexpr int kOffUnitMl = kOffUnit + kRows * kHD * 4;   // and [row]
   static constexpr int kSmem = kOffUnitMl + kRows * 8;
 };
-static_assert(Cfg<1>::kSmem <= 115712, "two CTAs per SM");
+static_assert(Cfg<1>::kSmem <= 115712 && Cfg<2>::kSmem <= 115712, "two CTAs per SM");
 
 struct Params {
   const bf16* q;
@@ -606,10 +608,10 @@ struct Edge {
 
 // kApart: the tensor cores add up the products of a tile, and the tiles' sums are added here, in fp32 with
 // rounding to nearest. A tensor core's own running sum is cut off, for codes always downwards: of 131072 keys
-// with 8 KV heads in one CTA's warps (5461 tiles each) that was 1.13 % of the result, and 0.06 % so; at 125
-// tiles a warp the two are alike (0.03 %, of which 0.02 are the probabilities' f16 rounding). Four rows keep
-// half of the sums and gain registers; eight rows pay 6 % of a tile (8 sequences of 5 rows, 4099 keys: 29.0
-// us, 27.2 without), and have it only where a warp's tiles may be more than kApartTiles.
+// with 8 KV heads in one CTA's warps (5461 tiles each) that was 1.13 % of the result, and 0.06 % so (0.02 %
+// with both signs); at 125 tiles a warp the two are alike. Four rows keep half of the sums and gain registers;
+// eight rows pay 9 % of a tile (8 sequences of 5 rows, 4099 keys: 29.0 us, 27.5 without), and have it only
+// where a warp's tiles may be more than kApartTiles.
 template <int NT, bool kApart>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, Cfg<NT>::kCtasPerSm) decode_kernel(const Params p) {
   using C = Cfg<NT>;
@@ -1118,8 +1120,8 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
     return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->num_qo_heads % a->num_kv_heads != 0) return SOLORT_ERR_INVALID_ARGUMENT;
   if (a->batch > 65535) return SOLORT_ERR_UNSUPPORTED;
-  // Four rows a block where they fit one, else eight: a tile of eight takes 1.25 of four's time (1217 and
-  // 977 cycles a scheduler), which two blocks of four would take twice.
+  // Four rows a block where they fit one, else eight: a tile of eight takes 1.4 of four's time (1392 and
+  // 979 cycles a scheduler, 1519 with kApart), which two blocks of four would take twice.
   const int64_t rows = static_cast<int64_t>(a->q_len) * (a->num_qo_heads / a->num_kv_heads);
   pl->nt = rows <= 4 ? 1 : 2;
   const int warps = pl->nt == 1 ? Cfg<1>::kWarps : Cfg<2>::kWarps;
@@ -1145,10 +1147,10 @@ int make_plan(const SolortInt4DecodeArgs* a, Plan* pl) {
   // resident at once, a warp's tiles are few, and no more than its share of the divided list and what the
   // division costs. k is what a warp's tiles and the cluster cost least with, in quarters of a tile; two
   // CTAs on an SM cost one more. 32 heads over 8, us with clusters of 1, 2, 4, 8 | divided:
-  //   1 x 256 keys   5.5  6.1  6.0  6.8 | 7.8      8 x 1024   11.1 10.0  9.8    - | 11.1
-  //   1 x 768        8.4  7.6  6.4  7.1 | 8.2      8 x 4096    33  22.1 16.0    - | 17.4
-  //   1 x 1536      12.8  9.8  7.9  7.2 | 7.8     16 x 1024   13.1 11.3    -    - | 12.9
-  //   1 x 4096      28   17.5 12.0  9.8 | 8.8     64 x 256    15.2    -    -    - | 15.9
+  //   1 x 256 keys   4.9  5.5  5.8  6.6 | 7.5      8 x 1024    9.9  8.7  9.2    - | 10.6
+  //   1 x 768        7.7  6.8  5.9  6.5 | 7.7      8 x 4096   28.6 18.2 15.9    - | 17.5
+  //   1 x 1536      12.4  9.2  7.2  6.6 | 7.8     16 x 1024   10.3 10.7    -    - | 12.6
+  //   1 x 4096      27.8 17.2 11.4  9.1 | 9.0     64 x 256       -    -    -    - | 16.5
   constexpr int kClusterCost[] = {0, 4, 5, 8};
   int64_t least = 0, steps = 0;
   for (int i = 0; (1 << i) <= kMostCluster && (units * a->batch << i) <= wave; ++i) {
@@ -1208,8 +1210,8 @@ int launch(const Params& prm, const Plan& pl, void* stream) {
   if (cudaLaunchKernelEx(&cfg, decode_kernel<NT, kApart>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;
   int rc = launch_status();
   if (rc != SOLORT_OK || pl.direct) return rc;
-  // Few rows have many parts each and want many warps (131072 keys, 32 rows: 8 warps 38.9 us, 2 warps
-  // 41.4); of many rows most are written already and want to leave (48 sequences, 1536 rows: 39.2 and 35.4).
+  // Few rows have many parts each and want many warps (131072 keys, 32 rows: 8 warps 38.8 us, 2 warps
+  // 41.1); of many rows most are written already and want to leave (48 sequences, 1536 rows: 38.1 and 35.4).
   const int rows = prm.batch * prm.q_len * prm.nh;
   cfg = pdl_config(dim3(rows), (rows <= pl.ctas ? kMergeWarps : 2) * 32, 0, stream, 1, attr);
   if (cudaLaunchKernelEx(&cfg, merge_kernel<NT>, prm) != cudaSuccess) return SOLORT_ERR_CUDA;

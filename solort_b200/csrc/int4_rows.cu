@@ -15,9 +15,9 @@
 // append's query CTAs go over several heads, with the tokens' RoPE rows in registers.
 //
 // All three are bound by the bytes they move, and for a decode step by their launch. 8 KV heads: storing
-// 16380 rows 17.0 us (5.2 TB/s), loading 32001 rows 30.1 us (5.7 TB/s), appending a prompt of 8190 tokens
-// with 32 query heads 38.1 us (4.8 TB/s: a token's RoPE rows wait for its position, and 96 registers
-// leave 20 warps an SM to hide that); one token's append 2.2 us.
+// 16380 rows 17.0 us (5.2 TB/s), loading 32001 rows 30.2 us (5.7 TB/s), appending a prompt of 8190 tokens
+// with 32 query heads 38.3 us (4.8 TB/s: a token's RoPE rows wait for its position, and 96 registers, with
+// 20 bytes a thread spilt, leave 20 warps an SM to hide that); one token's append 2.3 us.
 #include <math.h>
 
 #include "host_util.h"
@@ -32,8 +32,8 @@ namespace i4 {
 constexpr int kRowThreads = 128;
 constexpr int kRowsPerCta = kRowThreads / 8;
 constexpr int kGroupRowsPerCta = kRowThreads / 4;  // of four lanes a row
-// CTAs per SM from which a CTA takes more than one round of rows, or heads: 16380 rows stored 18.8 us with
-// 8, 17.6 with 16, 18.1 with 32; a prompt of 8190 tokens appended 38.1 us with 16, 41.7 with 32.
+// CTAs per SM from which a CTA takes more than one round of rows, or heads: a prompt of 8190 tokens appended
+// 38.4 us with 8 and with 16, 42.2 with 32; 16380 rows stored 16.6 us with 8, 17.0 with 16, 17.8 with 32.
 constexpr int kFullCtas = 16;
 
 struct Arena {
@@ -43,7 +43,7 @@ struct Arena {
   long long slots;  // num_pages * page_size
 };
 
-// The block of `slot`, or nullptr. A slot of -1 is padding and passes silently.
+// The block of `slot`, which is one of the arena's (row_there).
 __device__ __forceinline__ uint8_t* slot_block(const Arena& ar, long long slot, int head) {
   const int row = static_cast<int>(slot) & ar.page_mask;
   return ar.base + block_offset(slot >> ar.page_shift, row, head, ar.page_stride, ar.head_stride);
@@ -74,12 +74,7 @@ __device__ __forceinline__ f2 sum_of_products(f2 a, f2 b, f2 c, f2 d) {
               __fadd_rn(__fmul_rn(x.y, y.y), __fmul_rn(u.y, v.y)));
 }
 
-// The norm's sum of squares is fp32 for queries, which are rounded to bf16 at the end, and fp64 for
-// keys: a key's last fp32 bit can decide between two codes, and with the sum all but exact its value
-// does not depend on the order of the sum; its products and sums are each rounded on their own, without
-// contraction. Norm and rotation stay in fp32 with one rounding at the end (the bf16 cache's prologue
-// rounds after each step, as the reference's torch ops do).
-// True if `slot` (and `pos`) name a row; a bad one is reported.
+// True if `slot` (and `pos`) name a row; a bad one is reported, but for -1, which is padding.
 __device__ __forceinline__ bool row_there(long long slot, const Arena& ar, bool report, bool pos_ok = true) {
   if (slot == -1) return false;
   if (slot >= 0 && slot < ar.slots && pos_ok) return true;
@@ -87,6 +82,11 @@ __device__ __forceinline__ bool row_there(long long slot, const Arena& ar, bool 
   return false;
 }
 
+// The norm's sum of squares is fp32 for queries, which are rounded to bf16 at the end, and fp64 for
+// keys: a key's last fp32 bit can decide between two codes, and with the sum all but exact its value
+// does not depend on the order of the sum; its products and sums are each rounded on their own, without
+// contraction. Norm and rotation stay in fp32 with one rounding at the end (the bf16 cache's prologue
+// rounds after each step, as the reference's torch ops do).
 // Grid: (tokens, [query heads | key heads | value heads], p.heads each).
 __global__ void __launch_bounds__(kRowThreads, 5) append_kernel(const AppendParams p) {
   pdl_wait();
@@ -207,7 +207,6 @@ __global__ void __launch_bounds__(kRowThreads, 5) append_kernel(const AppendPara
 // Rows of a store, so that the row of a CTA's next round stays inside an int.
 constexpr int kMostStored = 1 << 30;
 
-// Eight CTAs an SM: 16380 rows 17.0 us; 17.6 with the 65 registers that the compiler takes, seven CTAs.
 struct StoreParams {
   const bf16* key;
   const bf16* value;
@@ -217,6 +216,8 @@ struct StoreParams {
   Arena ar;
 };
 
+// Eight CTAs an SM: 16380 rows 17.0 us; 17.6 with the 65 registers that the compiler takes, seven CTAs. A
+// row is read before its slot is known, a padded one too.
 __global__ void __launch_bounds__(kRowThreads, 8) store_kernel(const StoreParams p) {
   pdl_wait();
   const int g = threadIdx.x & 3;
@@ -243,7 +244,6 @@ __global__ void __launch_bounds__(kRowThreads, 8) store_kernel(const StoreParams
   }
 }
 
-// Sixteen CTAs an SM, all its warps: 32001 rows 30.1 us; 30.8 with two registers more, twelve CTAs.
 struct LoadParams {
   bf16* key;
   bf16* value;
@@ -253,6 +253,8 @@ struct LoadParams {
   Arena ar;
 };
 
+// Sixteen CTAs an SM, all its warps, with four bytes a thread spilt: 32001 rows 30.3 us; 31.0 with two
+// registers more, twelve CTAs.
 __global__ void __launch_bounds__(kRowThreads, 16) load_kernel(const LoadParams p) {
   pdl_wait();
   const int l8 = threadIdx.x & 7, t = l8 & 3, g = l8 >> 2;
@@ -381,8 +383,8 @@ extern "C" int solort_attn_qk_norm_rope_append_int4(const SolortInt4AppendArgs* 
   p.q_out = static_cast<bf16*>(a->q_out);
   p.qo_st = a->q_out_stride_token;
   p.qo_sh = a->q_out_stride_head;
-  // One head per CTA while the GPU is not full, and up to eight (prompt of 8190 tokens: at most four 41.7
-  // us, eight 38.1).
+  // One head per CTA while the GPU is not full, and up to eight (prompt of 8190 tokens: at most four 41.8
+  // us, eight 38.4).
   const int64_t x = (static_cast<int64_t>(a->num_tokens) + i4::kRowsPerCta - 1) / i4::kRowsPerCta;
   const int64_t full = static_cast<int64_t>(di.sm_count) * i4::kFullCtas;
   const int64_t per = x * (a->num_qo_heads + 2ll * a->num_kv_heads) / full;
